@@ -33,6 +33,7 @@ I = ctypes.c_int
 F = ctypes.c_float
 SZ = ctypes.c_size_t
 U64 = ctypes.c_uint64
+I64 = ctypes.c_int64
 
 # name -> argtypes (every function returns int)
 SIGNATURES = {
@@ -80,6 +81,17 @@ SIGNATURES = {
     "jsx_row_linear_allreduce_add": [P, P, P, P, P, I, I, I, P],
     "jsx_decode_step_workspace_size": [P, P],
     "jsx_decode_step": [P, P, P],
+    "jsx_kv4_page_bytes": [I, I, I, P],
+    "jsx_kv4_append": [P, P, I64, I64, I64, I, P, I, P, I, P, P, I, I, I, I, I, P],
+    "jsx_kv4_read": [P, I, P, I, P, P, P, P, I64, I64, I64, I, I, I, I, I, I, P],
+    "jsx_kv4_attn_workspace_size": [I, I, I, I, I, P],
+    "jsx_kv4_attn": [P, I64, P, I, P, I, P, P, P, I64, I, I, I, I, I, I, I, I, F, P, SZ, P],
+    "jsx_pages_workspace_size": [I, I, I, P],
+    "jsx_pages_fork": [P, P, P, P, P, P, P, I, I, I, P],
+    "jsx_pages_resize": [P, P, P, P, P, P, I, SZ, I, I, I, I, P, P, SZ, P],
+    "jsx_pages_compact": [P, P, P, P, I, SZ, P, P, P, I, I, I, P, SZ, P],
+    "jsx_verify_workspace_size": [I, I, I, P],
+    "jsx_verify_drafts": [P, I, I64, P, P, P, P, F, P, P, P, I, I, I, P, SZ, P],
     "jsx_comm_create": [I, I, I, I, U64, P],
     "jsx_comm_create_tiles": [I, I, I, I, U64, P],
     "jsx_comm_ipc_handle": [P, P],

@@ -1,0 +1,190 @@
+// Rows written to and read back from the 4-bit key/value pages (kv4.cuh).
+//
+// Append, per 16 values x of a row: s = e4m3(min(max |x| / 6, 448)), code =
+// e2m1(x / s) (0 where s is 0), both rounded to nearest even.  A bf16 value has
+// 8 significant bits and a scale 4, so a quotient is either exactly on a code's
+// rounding boundary or at least 2^-10 from it; x (1/s) is within 2^-21 of x / s.
+// Rounding it to multiples of 2^-13 (one fused multiply-add against 1536 and a
+// subtraction) therefore gives the codes of the exact quotient, without 16
+// divisions per group.  The largest magnitude is an integer maximum over the
+// bf16 bit patterns, where NaN is above infinity: a group with a NaN gets a NaN
+// scale and reads back as NaN; infinities saturate at 6 x 448.
+//
+// Both kernels are bound by memory: 32 bytes of bf16 per 9 bytes of page.  One
+// thread handles one group: two 16-byte accesses on the bf16 side, 8 bytes of
+// codes and one scale byte on the page side; the threads of a row are adjacent.
+#include "common.cuh"
+#include "kv4.cuh"
+#include "launch.cuh"
+
+namespace jsx {
+
+constexpr int kKv4Threads = 256;
+
+struct Kv4RowArgs {
+  bf16* k;  // append: read; read: written
+  bf16* v;
+  int64_t seq_stride, token_stride, head_stride;  // elements
+  int cache_rows;  // > 0: rows of a static cache, indexed by position; 0: one row per token of the call
+  uint8_t* pool;
+  const int32_t* table;
+  const int32_t* positions;
+  const int32_t* n_tokens;
+  int num_pages, slots, T, nkv, pt;
+  int64_t units;  // B * T * nkv * 2 * (D / 16)
+};
+
+// Where unit u lies: its 16 values in the row, and its block, token slot and group in the pool.
+struct Kv4Unit {
+  bf16* row;
+  uint8_t* codes;
+  uint8_t* scale;
+  bool inside;  // the row exists (token used, position inside the static cache)
+  bool paged;   // ... and has a page
+};
+
+template <int D>
+__device__ __forceinline__ Kv4Unit kv4_unit(const Kv4RowArgs& a, int64_t u) {
+  constexpr int NG = D / kKv4Group;
+  const int g = (int)(u % NG);
+  const int64_t r = u / NG;
+  const int which = (int)(r & 1);
+  const int64_t mh = r >> 1;
+  const int h = (int)(mh % a.nkv);
+  const int64_t m = mh / a.nkv;
+  const int b = (int)(m / a.T), i = (int)(m % a.T);
+  const int pos = a.positions[b] + i;
+  Kv4Unit x;
+  x.inside = (!a.n_tokens || i < a.n_tokens[b]) && pos >= 0 && (a.cache_rows == 0 || pos < a.cache_rows);
+  x.row = (which ? a.v : a.k) + b * a.seq_stride + (int64_t)(a.cache_rows ? pos : i) * a.token_stride +
+          h * a.head_stride + g * kKv4Group;
+  const int slot = pos / a.pt;
+  int page = -1;
+  if (x.inside && slot < a.slots) page = a.table[(int64_t)b * a.slots + slot];
+  x.paged = page >= 0 && page < a.num_pages;
+  const int t = pos - slot * a.pt;
+  uint8_t* block = a.pool + ((int64_t)page * a.nkv + h) * kv4_block_bytes(a.pt, D);
+  x.codes = block + (which ? kv4_off_v(a.pt, D) : 0) + t * (D / 2) + g * 8;
+  x.scale = block + (which ? kv4_off_vs(a.pt, D) : kv4_off_ks(a.pt, D)) + t * NG + g;
+  return x;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kKv4Threads) k_kv4_append(Kv4RowArgs a) {
+  pdl_wait();
+  const int64_t step = (int64_t)gridDim.x * kKv4Threads;
+  for (int64_t u = (int64_t)blockIdx.x * kKv4Threads + threadIdx.x; u < a.units; u += step) {
+    const Kv4Unit x = kv4_unit<D>(a, u);
+    if (!x.paged) continue;
+    const uint4 p0 = *reinterpret_cast<const uint4*>(x.row), p1 = *reinterpret_cast<const uint4*>(x.row + 8);
+    const uint32_t w[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+    uint32_t mx = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mx = __vmaxu2(mx, w[i] & 0x7fff7fffu);
+    const float top = __uint_as_float(max(mx & 0xffffu, mx >> 16) << 16);
+    const uint32_t sc = f32_to_e4m3(__fdiv_rn(top, 6.f));
+    const float s = __half2float(__ushort_as_half((unsigned short)(e4m3x2_to_h2(sc) & 0xffffu)));
+    const float inv = s == 0.f ? 0.f : __frcp_rn(s);
+    float q[2][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      q[i >> 2][2 * (i & 3)] = __fmaf_rn(bf_lo(w[i]), inv, 1536.f) - 1536.f;
+      q[i >> 2][2 * (i & 3) + 1] = __fmaf_rn(bf_hi(w[i]), inv, 1536.f) - 1536.f;
+    }
+    *reinterpret_cast<uint2*>(x.codes) = make_uint2(f32x8_to_e2m1(q[0]), f32x8_to_e2m1(q[1]));
+    *x.scale = (uint8_t)sc;
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kKv4Threads) k_kv4_read(Kv4RowArgs a) {
+  pdl_wait();
+  const int64_t step = (int64_t)gridDim.x * kKv4Threads;
+  for (int64_t u = (int64_t)blockIdx.x * kKv4Threads + threadIdx.x; u < a.units; u += step) {
+    const Kv4Unit x = kv4_unit<D>(a, u);
+    if (!x.inside) continue;
+    uint32_t o[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+    if (x.paged) {
+      const uint2 c = *reinterpret_cast<const uint2*>(x.codes);
+      const uint32_t sc = *x.scale;
+      const uint32_t s2 = e4m3x2_to_h2(sc | (sc << 8));
+      uint32_t h[8];
+      e2m1x8_to_h2(c.x, reinterpret_cast<uint32_t(&)[4]>(h[0]));
+      e2m1x8_to_h2(c.y, reinterpret_cast<uint32_t(&)[4]>(h[4]));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t y = hmul2_u(h[i], s2);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&y));
+        o[i] = pack2(f.x, f.y);
+      }
+    }
+    *reinterpret_cast<uint4*>(x.row) = make_uint4(o[0], o[1], o[2], o[3]);
+    *reinterpret_cast<uint4*>(x.row + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+  }
+}
+
+static int kv4_rows(bool append, const void* k, const void* v, int64_t seq_stride, int64_t token_stride,
+                    int64_t head_stride, int cache_rows, const void* pool, int num_pages, const int32_t* table,
+                    int table_slots, const int32_t* positions, const int32_t* n_tokens, int B, int T, int nkv,
+                    int head_dim, int page_tokens, void* stream) {
+  JSX_REQUIRE(k && v && positions, "null pointer argument");
+  JSX_KV4_REQUIRE(pool, num_pages, table, table_slots, nkv, head_dim, page_tokens);
+  JSX_REQUIRE(B >= 1 && T >= 1 && cache_rows >= 0, "B=%d T=%d cache_rows=%d", B, T, cache_rows);
+  JSX_REQUIRE(aligned16(k) && aligned16(v) && seq_stride % 8 == 0 && token_stride % 8 == 0 && head_stride % 8 == 0,
+              "rows must be 16-byte aligned");
+  JSX_REQUIRE(seq_stride >= 0 && token_stride >= 0 && head_stride >= 0, "negative stride");
+  Kv4RowArgs a;
+  a.k = (bf16*)const_cast<void*>(k);
+  a.v = (bf16*)const_cast<void*>(v);
+  a.seq_stride = seq_stride;
+  a.token_stride = token_stride;
+  a.head_stride = head_stride;
+  a.cache_rows = cache_rows;
+  a.pool = (uint8_t*)const_cast<void*>(pool);
+  a.table = table;
+  a.positions = positions;
+  a.n_tokens = n_tokens;
+  a.num_pages = num_pages;
+  a.slots = table_slots;
+  a.T = T;
+  a.nkv = nkv;
+  a.pt = page_tokens;
+  a.units = (int64_t)B * T * nkv * 2 * (head_dim / kKv4Group);
+  const int64_t blocks = (a.units + kKv4Threads - 1) / kKv4Threads;
+  const dim3 grid((unsigned)(blocks < 8ll * sm_count() ? blocks : 8ll * sm_count()));
+  auto kern = append ? (head_dim == 128 ? k_kv4_append<128> : k_kv4_append<64>)
+                     : (head_dim == 128 ? k_kv4_read<128> : k_kv4_read<64>);
+  JSX_CUDA(launch_kernel(kern, grid, dim3(kKv4Threads), 0, (cudaStream_t)stream, a));
+  return JSX_OK;
+}
+
+}  // namespace jsx
+
+using namespace jsx;
+
+extern "C" int jsx_kv4_page_bytes(int nkv, int head_dim, int page_tokens, size_t* bytes) {
+  JSX_REQUIRE(bytes && nkv >= 1, "bad arguments");
+  JSX_REQUIRE(kv4_page_tokens_ok(page_tokens), "page_tokens=%d is not 16, 32, 64 or 128", page_tokens);
+  if (head_dim != 64 && head_dim != 128) {
+    set_error("head_dim=%d (the 4-bit cache takes 64 and 128)", head_dim);
+    return JSX_ENOTSUP;
+  }
+  *bytes = (size_t)nkv * kv4_block_bytes(page_tokens, head_dim);
+  return JSX_OK;
+}
+
+extern "C" int jsx_kv4_append(const void* k, const void* v, int64_t seq_stride, int64_t token_stride,
+                              int64_t head_stride, int cache_rows, void* pool, int num_pages, const int32_t* table,
+                              int table_slots, const int32_t* positions, const int32_t* n_tokens, int B, int T,
+                              int nkv, int head_dim, int page_tokens, void* stream) {
+  return kv4_rows(true, k, v, seq_stride, token_stride, head_stride, cache_rows, pool, num_pages, table, table_slots,
+                  positions, n_tokens, B, T, nkv, head_dim, page_tokens, stream);
+}
+
+extern "C" int jsx_kv4_read(const void* pool, int num_pages, const int32_t* table, int table_slots,
+                            const int32_t* positions, const int32_t* n_tokens, void* k, void* v, int64_t seq_stride,
+                            int64_t token_stride, int64_t head_stride, int cache_rows, int B, int T, int nkv,
+                            int head_dim, int page_tokens, void* stream) {
+  return kv4_rows(false, k, v, seq_stride, token_stride, head_stride, cache_rows, pool, num_pages, table, table_slots,
+                  positions, n_tokens, B, T, nkv, head_dim, page_tokens, stream);
+}

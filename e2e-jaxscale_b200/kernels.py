@@ -501,6 +501,220 @@ def moe_gate(x, w_nk, k, scale, norm=True, correction_bias=None, logits_given=Fa
     return topk_w, topk_i
 
 
+# ---- paged 4-bit key/value cache (jsx_kv4_*, jsx_pages_*) ----------------------
+I32 = torch.int32
+
+
+def _kv4_pool(pool, table, positions, n_tokens, head_dim):
+    """(num_pages, nkv, page_tokens, slots, B) of one layer's pool [num_pages, nkv, block]."""
+    _need(pool, "pool", torch.uint8)
+    _need(table, "table", I32)
+    _need(positions, "positions", I32)
+    _opt(n_tokens, "n_tokens", I32)
+    if pool.dim() != 3 or table.dim() != 2:
+        raise ValueError("pool must be [num_pages, nkv, block] (one layer) and table [B, slots]")
+    P_, nkv, block = pool.shape
+    B, slots = table.shape
+    pt, rest = divmod(block * 8, 9 * head_dim)
+    if rest:
+        raise ValueError(f"a block of {block} bytes is not a whole number of rows of head_dim {head_dim}")
+    if positions.numel() != B or (n_tokens is not None and n_tokens.numel() != B):
+        raise ValueError(f"positions and n_tokens must have one entry per sequence ({B})")
+    return P_, nkv, pt, slots, B
+
+
+def kv4_page_bytes(nkv, head_dim, page_tokens) -> int:
+    n = ctypes.c_size_t(0)
+    call("jsx_kv4_page_bytes", nkv, head_dim, page_tokens, ctypes.byref(n))
+    return n.value
+
+
+def _kv4_rows(k, v, B, T, nkv):
+    """Strides and cache rows of k and v: [B, L, nkv, hd] (a static cache, rows by position) or
+    [B * T, nkv, hd] (one row per token; the tokens may be strided, as slices of a fused q/k/v are)."""
+    if k.shape != v.shape or k.stride() != v.stride() or k.dtype != BF16 or v.dtype != BF16:
+        raise ValueError("k and v must be bf16 of one shape and layout")
+    if not (k.is_cuda and v.is_cuda):
+        raise ValueError("k and v must be CUDA tensors")
+    st = k.stride()
+    if st[-1] != 1 or k.shape[-2] != nkv:
+        raise ValueError(f"rows must be [{nkv} kv heads, head_dim] with unit stride")
+    if k.dim() == 4:
+        if k.shape[0] != B:
+            raise ValueError(f"a static cache of {k.shape[0]} sequences, page table of {B}")
+        return st[0], st[1], st[2], k.shape[1]
+    if k.dim() != 3 or k.shape[0] != B * T:
+        raise ValueError(f"k and v must be [{B} * {T}, nkv, head_dim] or [{B}, rows, nkv, head_dim]")
+    return st[0] * T, st[0], st[1], 0
+
+
+def kv4_append(k, v, pool, table, positions, tokens_per_seq=1, n_tokens=None):
+    """Quantise T rows per sequence into the pages at positions[b] .. + T - 1 (include/jsx.h
+    jsx_kv4_append).  k, v: [B * T, nkv, hd], or a static cache [B, L, nkv, hd] read by position."""
+    hd = k.shape[-1]
+    P_, nkv, pt, slots, B = _kv4_pool(pool, table, positions, n_tokens, hd)
+    ss, ts, hs, rows = _kv4_rows(k, v, B, tokens_per_seq, nkv)
+    call("jsx_kv4_append", k.data_ptr(), v.data_ptr(), ss, ts, hs, rows, pool.data_ptr(), P_, table.data_ptr(), slots,
+         positions.data_ptr(), None if n_tokens is None else n_tokens.data_ptr(), B, tokens_per_seq, nkv, hd, pt,
+         _stream())
+
+
+def kv4_read(pool, table, positions, k, v, tokens_per_seq=1, n_tokens=None):
+    """Write the stored values of the same tokens to rows of k and v (layouts as kv4_append)."""
+    hd = k.shape[-1]
+    P_, nkv, pt, slots, B = _kv4_pool(pool, table, positions, n_tokens, hd)
+    ss, ts, hs, rows = _kv4_rows(k, v, B, tokens_per_seq, nkv)
+    call("jsx_kv4_read", pool.data_ptr(), P_, table.data_ptr(), slots, positions.data_ptr(),
+         None if n_tokens is None else n_tokens.data_ptr(), k.data_ptr(), v.data_ptr(), ss, ts, hs, rows, B,
+         tokens_per_seq, nkv, hd, pt, _stream())
+
+
+def kv4_attn_workspace(B, T, nq, nkv, head_dim, device) -> torch.Tensor:
+    n = ctypes.c_size_t(0)
+    call("jsx_kv4_attn_workspace_size", B, T, nq, nkv, head_dim, ctypes.byref(n))
+    return torch.zeros(n.value, dtype=torch.uint8, device=device)
+
+
+def kv4_attn(q, pool, table, positions, head_dim, workspace, scale=None, tokens_per_seq=1, n_tokens=None, window=0,
+             sinks=0, out=None):
+    """Attention of T tokens per sequence over the 4-bit pages: q [B * T, nq * hd] (token rows may
+    be strided) -> out [B * T, nq * hd].  window 0: every earlier row is visible; else the last
+    `window` rows and the first `sinks` rows (include/jsx.h jsx_kv4_attn)."""
+    P_, nkv, pt, slots, B = _kv4_pool(pool, table, positions, n_tokens, head_dim)
+    _need(workspace, "workspace", torch.uint8)
+    T = tokens_per_seq
+    if q.dim() != 2 or q.shape[0] != B * T or q.shape[1] % head_dim or q.stride(1) != 1:
+        raise ValueError(f"q must be [{B} * {T}, heads * {head_dim}] with unit stride in a row")
+    if not q.is_cuda or q.dtype != BF16:
+        raise TypeError("q must be a bf16 CUDA tensor")
+    if out is None:
+        out = torch.empty(q.shape, dtype=BF16, device=q.device)
+    elif out.shape != q.shape or out.dtype != BF16 or out.stride(1) != 1 or not out.is_cuda:
+        raise ValueError("out must be a bf16 CUDA tensor of q's shape")
+    call("jsx_kv4_attn", q.data_ptr(), q.stride(0), pool.data_ptr(), P_, table.data_ptr(), slots, positions.data_ptr(),
+         None if n_tokens is None else n_tokens.data_ptr(), out.data_ptr(), out.stride(0), B, T,
+         q.shape[1] // head_dim, nkv, head_dim, pt, window, sinks, head_dim ** -0.5 if scale is None else scale,
+         workspace.data_ptr(), workspace.numel(), _stream())
+    return out
+
+
+def pages_workspace(sequences, slots, num_pages, device) -> torch.Tensor:
+    n = ctypes.c_size_t(0)
+    call("jsx_pages_workspace_size", sequences, slots, num_pages, ctypes.byref(n))
+    return torch.empty(n.value, dtype=torch.uint8, device=device)
+
+
+def _pages(table, held, refs):
+    _need(table, "table", I32)
+    _need(held, "held", I32)
+    _need(refs, "refs", I32)
+    if table.dim() != 2 or held.numel() != table.shape[0]:
+        raise ValueError("table must be [S, slots] and held [S]")
+    return table.shape[0], table.shape[1], refs.numel()
+
+
+def _pages_pool(pool, num_pages):
+    """(layers, bytes of a page) of a pool [layers, num_pages, ...] or [num_pages, nkv, block]."""
+    _need(pool, "pool", torch.uint8)
+    layers = pool.shape[0] if pool.dim() == 4 else 1
+    if pool.dim() not in (3, 4) or pool.shape[-3] != num_pages:
+        raise ValueError(f"pool must be [layers, {num_pages}, nkv, block] or [{num_pages}, nkv, block]")
+    return layers, pool.shape[-1] * pool.shape[-2]
+
+
+def pages_fork(table, held, refs, parent, table_out=None, held_out=None, refs_out=None):
+    """Row b becomes row parent[b] (-1: empty); pages are shared.  Returns (table, held, refs)."""
+    S, slots, P_ = _pages(table, held, refs)
+    _need(parent, "parent", I32)
+    if parent.numel() != S:
+        raise ValueError(f"parent must have one entry per sequence ({S})")
+    table_out = torch.empty_like(table) if table_out is None else _need(table_out, "table_out", I32)
+    held_out = torch.empty_like(held) if held_out is None else _need(held_out, "held_out", I32)
+    refs_out = torch.empty_like(refs) if refs_out is None else _need(refs_out, "refs_out", I32)
+    if table_out.shape != table.shape or held_out.numel() != S or refs_out.numel() != P_:
+        raise ValueError("table_out, held_out and refs_out must have the shapes of table, held and refs")
+    call("jsx_pages_fork", table.data_ptr(), held.data_ptr(), refs.data_ptr(), parent.data_ptr(), table_out.data_ptr(),
+         held_out.data_ptr(), refs_out.data_ptr(), S, slots, P_, _stream())
+    return table_out, held_out, refs_out
+
+
+def pages_resize(table, held, refs, keep, need, pool, page_tokens, workspace, missing=None):
+    """In place: row b keeps its first keep[b] tokens and has pages of its own for need[b]
+    (include/jsx.h jsx_pages_resize).  Returns missing, int32 [1] on the device: 0, or how many
+    pages there were too few (nothing is changed then)."""
+    S, slots, P_ = _pages(table, held, refs)
+    _need(keep, "keep", I32)
+    _need(need, "need", I32)
+    _need(workspace, "workspace", torch.uint8)
+    if keep.numel() != S or need.numel() != S:
+        raise ValueError(f"keep and need must have one entry per sequence ({S})")
+    layers, page_bytes = _pages_pool(pool, P_)
+    missing = torch.empty(1, dtype=I32, device=table.device) if missing is None else _need(missing, "missing", I32)
+    call("jsx_pages_resize", table.data_ptr(), held.data_ptr(), refs.data_ptr(), keep.data_ptr(), need.data_ptr(),
+         pool.data_ptr(), layers, page_bytes, S, slots, P_, page_tokens, missing.data_ptr(), workspace.data_ptr(),
+         workspace.numel(), _stream())
+    return missing
+
+
+def pages_compact(table, held, refs, pool, workspace, table_out=None, refs_out=None, remap=None):
+    """Live pages move to the lowest numbers (include/jsx.h jsx_pages_compact); the outputs may be
+    table and refs themselves.  Returns (table, refs, remap)."""
+    S, slots, P_ = _pages(table, held, refs)
+    _need(workspace, "workspace", torch.uint8)
+    layers, page_bytes = _pages_pool(pool, P_)
+    table_out = torch.empty_like(table) if table_out is None else _need(table_out, "table_out", I32)
+    refs_out = torch.empty_like(refs) if refs_out is None else _need(refs_out, "refs_out", I32)
+    remap = torch.empty_like(refs) if remap is None else _need(remap, "remap", I32)
+    if table_out.shape != table.shape or refs_out.numel() != P_ or remap.numel() != P_:
+        raise ValueError("table_out, refs_out and remap must have the shapes of table, refs and refs")
+    call("jsx_pages_compact", table.data_ptr(), held.data_ptr(), refs.data_ptr(), pool.data_ptr(), layers, page_bytes,
+         table_out.data_ptr(), refs_out.data_ptr(), remap.data_ptr(), S, slots, P_, workspace.data_ptr(),
+         workspace.numel(), _stream())
+    return table_out, refs_out, remap
+
+
+# ---- drafted tokens (jsx_verify_drafts) ----------------------------------------
+def verify_workspace(B, T, V, device) -> torch.Tensor:
+    n = ctypes.c_size_t(0)
+    call("jsx_verify_workspace_size", B, T, V, ctypes.byref(n))
+    return torch.empty(n.value, dtype=torch.uint8, device=device)
+
+
+def verify_drafts(logits, draft_ids, uniforms, workspace, draft_probs=None, n_draft=None, temperature=1.0,
+                  accepted=None, tokens=None, accept_prob=None):
+    """Accept or refuse drafted tokens and draw one more (include/jsx.h jsx_verify_drafts).
+    logits [B, T + 1, V] bf16 or f32 (rows may be strided), draft_ids [B, T] int32, uniforms
+    [B, T + 1] f32, draft_probs [B, T, V] f32 or None (certain drafts), n_draft [B] int32 or None.
+    Returns (accepted [B], tokens [B, T + 1], accept_prob [B, T])."""
+    if logits.dim() != 3 or not logits.is_cuda or logits.dtype not in (BF16, torch.float32):
+        raise ValueError("logits must be a [B, T + 1, V] bf16 or f32 CUDA tensor")
+    B, T, V = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+    sb, sr, sv = logits.stride()
+    if sv != 1 or (B > 1 and sb != sr * (T + 1)):
+        raise ValueError("logits rows must be evenly spaced, with unit stride in a row")
+    _need(draft_ids, "draft_ids", I32)
+    _opt(uniforms, "uniforms", torch.float32)
+    _opt(draft_probs, "draft_probs", torch.float32)
+    _opt(n_draft, "n_draft", I32)
+    _need(workspace, "workspace", torch.uint8)
+    if (draft_ids.numel() != B * T or (uniforms is not None and uniforms.numel() != B * (T + 1))
+            or (n_draft is not None and n_draft.numel() != B)
+            or (draft_probs is not None and draft_probs.numel() != B * T * V)):
+        raise ValueError("draft_ids [B, T], uniforms [B, T + 1], draft_probs [B, T, V] and n_draft [B] must match logits")
+    dev = logits.device
+    accepted = torch.empty(B, dtype=I32, device=dev) if accepted is None else _need(accepted, "accepted", I32)
+    tokens = torch.empty((B, T + 1), dtype=I32, device=dev) if tokens is None else _need(tokens, "tokens", I32)
+    accept_prob = (torch.empty((B, T), dtype=torch.float32, device=dev) if accept_prob is None
+                   else _need(accept_prob, "accept_prob", torch.float32))
+    if accepted.numel() != B or tokens.numel() != B * (T + 1) or accept_prob.numel() != B * T:
+        raise ValueError("accepted [B], tokens [B, T + 1] and accept_prob [B, T] must match logits")
+    call("jsx_verify_drafts", logits.data_ptr(), int(logits.dtype == torch.float32), sr, draft_ids.data_ptr(),
+         None if draft_probs is None else draft_probs.data_ptr(), None if n_draft is None else n_draft.data_ptr(),
+         None if uniforms is None else uniforms.data_ptr(), temperature, accepted.data_ptr(), tokens.data_ptr(),
+         accept_prob.data_ptr(), B, T, V, workspace.data_ptr(), workspace.numel(), _stream())
+    return accepted, tokens, accept_prob
+
+
 # ---- whole decode step (jsx_decode_step) --------------------------------------
 class LayerWeights(ctypes.Structure):
     """jsx_layer_weights (include/jsx.h)."""

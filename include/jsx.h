@@ -410,6 +410,104 @@ int jsx_moe_gate(const void* x, const void* w_nk, const float* correction_bias, 
                  int32_t* topk_idx, int N, int H, int E, int k, float scale, int norm,
                  void* stream);
 
+/* ---- paged 4-bit key/value cache -------------------------------------------
+ * No counterpart in the reference, whose cache is a static bf16 array
+ * (layers/kv_cache.py:16-61).  A pool is [num_pages][nkv][block] bytes; a page
+ * holds page_tokens (16, 32, 64 or 128) rows of K and V of every kv head, and
+ * its block for one head is
+ *   K codes [pt][hd/2] | V codes [pt][hd/2] | K scales [pt][hd/16] | V scales [pt][hd/16]
+ * with two e2m1 codes per byte (even dimension in the low half) and one e4m3
+ * scale per 16 values of a row: 4.5 bits per value.  head_dim 64 or 128
+ * (JSX_ENOTSUP otherwise).  page_table [B][table_slots] int32 names the page of
+ * every page_tokens tokens of a sequence; an entry outside [0, num_pages) is a
+ * missing page: its tokens are not written, read as zero, and are not visible.
+ * Token i < tokens_per_seq (T) of sequence b is at position positions[b] + i;
+ * n_tokens[b] (nullable: T) is how many of its T tokens sequence b uses, and
+ * negative positions are unused too. */
+int jsx_kv4_page_bytes(int nkv, int head_dim, int page_tokens, size_t* bytes);
+/* Quantises rows of k and v (bf16) into the pages: per 16 values x of a row,
+ * scale = e4m3(min(max |x| / 6, 448)) and code = e2m1(x / scale), rounded to
+ * nearest even (code 0 where the scale is 0; a NaN makes its group NaN).
+ * Strides in elements, multiples of 8; rows 16-byte aligned.  cache_rows 0: the
+ * row of token i of sequence b is at b * seq_stride + i * token_stride (+ head *
+ * head_stride).  cache_rows > 0: k and v are a static cache of that many rows
+ * per sequence and the row is at b * seq_stride + position * token_stride. */
+int jsx_kv4_append(const void* k, const void* v, int64_t seq_stride, int64_t token_stride,
+                   int64_t head_stride, int cache_rows, void* pool, int num_pages,
+                   const int32_t* page_table, int table_slots, const int32_t* positions,
+                   const int32_t* n_tokens, int B, int T, int nkv, int head_dim, int page_tokens,
+                   void* stream);
+/* The reverse: writes the stored values (exact in bf16) of the same tokens to rows of k and v. */
+int jsx_kv4_read(const void* pool, int num_pages, const int32_t* page_table, int table_slots,
+                 const int32_t* positions, const int32_t* n_tokens, void* k, void* v,
+                 int64_t seq_stride, int64_t token_stride, int64_t head_stride, int cache_rows,
+                 int B, int T, int nkv, int head_dim, int page_tokens, void* stream);
+/* Attention of T tokens per sequence over the pages: query row (b, i) at
+ * position p sees cache row j when j <= p and (window == 0 or j > p - window or
+ * j < sinks); out = softmax(scale q.k) v over the visible rows, 0 when there is
+ * none.  q and out [B * T][nq][head_dim] bf16 with token strides q_stride and
+ * out_stride (elements, multiples of 8); query head h reads kv head h / (nq / nkv).
+ * workspace: jsx_kv4_attn_workspace_size bytes, 16-byte aligned, zero-filled once
+ * (left zeroed by every call). */
+int jsx_kv4_attn_workspace_size(int B, int T, int nq, int nkv, int head_dim, size_t* bytes);
+int jsx_kv4_attn(const void* q, int64_t q_stride, const void* pool, int num_pages,
+                 const int32_t* page_table, int table_slots, const int32_t* positions,
+                 const int32_t* n_tokens, void* out, int64_t out_stride, int B, int T, int nq,
+                 int nkv, int head_dim, int page_tokens, int window, int sinks, float scale,
+                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* Pages of a paged cache, kept on the device: table [S][slots] names the pages of
+ * every sequence, held [S] how many slots of a row are in use, refs [num_pages]
+ * how many holders a page has (0: free; a caller may add its own holds).
+ * workspace: jsx_pages_workspace_size bytes, 16-byte aligned, contents free.
+ * At most 2^15 sequences and 2^30 table entries. */
+int jsx_pages_workspace_size(int sequences, int slots, int num_pages, size_t* bytes);
+/* Row b of the outputs is row parent[b] (any other value than 0..S-1: empty);
+ * pages are shared, not copied, and refs_out counts the new holders.  parent[b]
+ * == b keeps a row, several rows may have one parent.  refs_out may be refs;
+ * table_out and held_out are other arrays than table and held. */
+int jsx_pages_fork(const int32_t* table, const int32_t* held, const int32_t* refs,
+                   const int32_t* parent, int32_t* table_out, int32_t* held_out, int32_t* refs_out,
+                   int sequences, int slots, int num_pages, void* stream);
+/* Row b keeps its first keep[b] tokens (at most need[b]) and gets pages for need[b]
+ * tokens.  Pages from keep[b] on that others hold too are replaced by free ones
+ * (their bytes are copied in every layer of pool [layers][num_pages][page_bytes] if
+ * they hold kept tokens); pages beyond need[b] are given back.  Free pages are taken
+ * lowest first, in sequence and slot order, from those that were free before the
+ * call.  *missing = 0, or, with nothing changed, how many pages there were too few
+ * (free ones or table slots). */
+int jsx_pages_resize(int32_t* table, int32_t* held, int32_t* refs, const int32_t* keep,
+                     const int32_t* need, void* pool, int layers, size_t page_bytes, int sequences,
+                     int slots, int num_pages, int page_tokens, int32_t* missing, void* workspace,
+                     size_t workspace_bytes, void* stream);
+/* Moves the n live pages to 0..n-1: live pages with numbers from n on move, in
+ * ascending order, into the free ones below n.  remap[num_pages] = new number of
+ * every live page, -1 of free ones.  table_out may be table and refs_out refs. */
+int jsx_pages_compact(const int32_t* table, const int32_t* held, const int32_t* refs, void* pool,
+                      int layers, size_t page_bytes, int32_t* table_out, int32_t* refs_out,
+                      int32_t* remap, int sequences, int slots, int num_pages, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* Verification of drafted tokens.  logits [B][T + 1][V] bf16 (or f32 when
+ * logits_f32), rows row_stride elements apart: row i is the target's prediction
+ * after i drafted tokens.  p = softmax(logits / temperature); draft_ids [B][T]
+ * drawn from draft_probs [B][T][V] f32 (NULL: certain drafts, q = 1), n_draft[B]
+ * (NULL: T) drafts per sequence, uniforms [B][T + 1] f32 in [0, 1).  Draft i is
+ * accepted while uniforms[i] q_i(x_i) < p_i(x_i); accepted[b] counts them;
+ * tokens[b] = the accepted drafts, one more token drawn with uniforms[T] from
+ * max(p - q, 0) after a refusal (q = the refused token alone without draft_probs)
+ * or from p, then -1.  accept_prob [B][T] = min(1, p / q), 0 for unused drafts and
+ * ids outside [0, V).  temperature 0: greedy (p = 1 at the first maximum; uniforms
+ * may be NULL).  Sums are over integers (weights of 2^-40), so the tokens do not
+ * depend on the order of execution.  NaN logits have no mass; a row without a
+ * finite maximum accepts nothing and draws -1.  0 <= T <= 31, V <= 2^20. */
+int jsx_verify_workspace_size(int B, int T, int V, size_t* bytes);
+int jsx_verify_drafts(const void* logits, int logits_f32, int64_t row_stride,
+                      const int32_t* draft_ids, const float* draft_probs, const int32_t* n_draft,
+                      const float* uniforms, float temperature, int32_t* accepted, int32_t* tokens,
+                      float* accept_prob, int B, int T, int V, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 /* ---- tensor-parallel group (utils/mesh_utils.py:8-45 "tensor" axis) ------- */
 /* Allocates this rank's symmetric buffer on the current device: fp32 partial
  * slots for up to max_tokens x hidden, flags and state.  timeout_ns bounds
