@@ -781,6 +781,7 @@ namespace jsx {
 int read_clear_step_error(uint32_t* out);  // decode_step.cu
 int read_clear_tc_error(uint32_t* out);    // tc_gemm.cu
 int read_clear_wide_error(uint32_t* out);  // tc_wide.cu
+int read_clear_kv4_error(uint32_t* out);   // kv4_attn.cu
 }
 
 extern "C" int jsx_device_error(int* status) {
@@ -800,6 +801,9 @@ extern "C" int jsx_device_error(int* status) {
   uint32_t u = 0;
   st = jsx::read_clear_wide_error(&u);
   if (st != JSX_OK) return st;
-  *status = (v | w | t | u) ? JSX_ETIMEDOUT : JSX_OK;
+  uint32_t x = 0;
+  st = jsx::read_clear_kv4_error(&x);
+  if (st != JSX_OK) return st;
+  *status = (v | w | t | u | x) ? JSX_ETIMEDOUT : JSX_OK;
   return JSX_OK;
 }

@@ -54,7 +54,7 @@ int jsx_device_sm_count(int* out);
 int jsx_set_launch_flags(int flags);
 int jsx_get_launch_flags(void);
 /* Reads and clears the device error words of the streaming GEMV, of the
- * whole-step kernel and of the tensor-core projections: a bounded pipeline or
+ * whole-step kernel, of the tensor-core projections and of jsx_kv4_attn: a bounded pipeline or
  * grid-barrier wait that gave up (the kernel then finished without its
  * result) reports JSX_ETIMEDOUT.
  * Synchronous (a device copy). */
@@ -423,7 +423,7 @@ int jsx_moe_gate(const void* x, const void* w_nk, const float* correction_bias, 
  * missing page: its tokens are not written, read as zero, and are not visible.
  * Token i < tokens_per_seq (T) of sequence b is at position positions[b] + i;
  * n_tokens[b] (nullable: T) is how many of its T tokens sequence b uses, and
- * negative positions are unused too. */
+ * negative positions are unused too.  Positions are below 2^30. */
 int jsx_kv4_page_bytes(int nkv, int head_dim, int page_tokens, size_t* bytes);
 /* Quantises rows of k and v (bf16) into the pages: per 16 values x of a row,
  * scale = e4m3(min(max |x| / 6, 448)) and code = e2m1(x / scale), rounded to
