@@ -6,7 +6,7 @@
 // present; o = sum_j softmax_j(scale q . k_j) v_j, and 0 when it sees nothing.
 //
 // Split.  The G = nq / nkv query heads of a kv head times the T tokens are its rows;
-// an item is one (sequence, kv head, tile of 16 rows), a chunk 64 cache rows.  The
+// an item is one (sequence, kv head, tile of 16 rows), a chunk 128 cache rows.  The
 // chunks of all items form one list, cut into equal ranges, one per CTA, so a long
 // sequence among short ones loads every SM alike; lengths are read on the device.  A
 // CTA that holds only part of an item writes (max, sum, unnormalised output) to the
@@ -14,8 +14,8 @@
 // order: the result does not depend on who is last.
 //
 // Inside a CTA one warp copies a chunk's codes and scales into a ring of shared-memory
-// stages (cp.async.bulk, 9 KB per stage at head_dim 128) and four warps take 16 of its
-// 64 cache rows each, with their own running maximum and sum.  S = Q K^T and O += P V run on
+// stages (cp.async.bulk, 18 KB per stage at head_dim 128) and four warps take 32 of its
+// 128 cache rows each, with their own running maximum and sum.  S = Q K^T and O += P V run on
 // mma.sync m16n8k16 f16: a stored value (at most 6 significant bits) is exact in f16,
 // q is scaled per row by a power of two into f16's range (also exact, short of values
 // 2^-23 below the row's largest), P is rounded to f16, everything else is fp32.
@@ -34,10 +34,12 @@
 namespace jsx {
 
 constexpr int kKaRows = 16;     // query rows per item
-constexpr int kKaChunk = 64;    // cache rows per stage
-constexpr int kKaWarps = 4;     // computing warps, 16 cache rows of a chunk each
+constexpr int kKaChunk = 128;   // cache rows per stage
+constexpr int kKaWarps = 4;     // computing warps, 32 cache rows of a chunk each
+constexpr int kKaKeys = kKaChunk / kKaWarps;
+constexpr int kKaPieces = kKaKeys / 16;
 constexpr int kKaThreads = (kKaWarps + 1) * 32;
-constexpr int kKaStages = 4;
+constexpr int kKaStages = 3;
 constexpr int kKaFan = 16;      // parts joined at once
 constexpr int kKaLevels = 3;    // 16^3 parts of an item at most
 constexpr int kKaListMax = 1024;  // (sequence, row tile) pairs up to which the chunk list is cut into ranges
@@ -65,7 +67,8 @@ struct KaArgs {
   uint32_t* arrived;  // [kKaLevels][2 x CTAs], zero between calls
   int num_pages, slots, B, T, nkv, G, tiles, pt, window, sinks;
   int listed;  // chunk list cut into ranges; else whole items per CTA
-  float scale_log2;
+  uint32_t negate;   // 0x80000000 when the scale is negative
+  float scale_log2;  // its magnitude x log2(e)
 };
 
 template <int D>
@@ -203,7 +206,7 @@ __device__ __forceinline__ bool ka_nan_scale(uint32_t s) { return (s & 0x7fu) ==
 // One row's D / 4 values of q at `p` as f16 pairs, scaled by the power of two that brings
 // the row's largest magnitude to 2^8 .. 2^9; returns what undoes it.
 template <int N>
-__device__ __forceinline__ float ka_load_q(const bf16* p, bool live, uint32_t (&h)[N / 2]) {
+__device__ __forceinline__ float ka_load_q(const bf16* p, bool live, uint32_t (&h)[N / 2], uint32_t negate) {
   uint32_t w[N / 2];
 #pragma unroll
   for (int i = 0; i < N / 8; ++i) {
@@ -221,7 +224,7 @@ __device__ __forceinline__ float ka_load_q(const bf16* p, bool live, uint32_t (&
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   const int e = (int)(top >> 7);  // exponent field of the largest
   const int f = e == 255 ? 127 : min(262 - e, 254);
-  const float mul = __uint_as_float((uint32_t)f << 23);
+  const float mul = __uint_as_float((uint32_t)f << 23 | negate);
 #pragma unroll
   for (int i = 0; i < N / 2; ++i) h[i] = ka_h2(bf_lo(w[i]) * mul, bf_hi(w[i]) * mul);
   return f == 254 ? 0x1p-127f : __uint_as_float((uint32_t)(254 - f) << 23);
@@ -350,7 +353,7 @@ __global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
         const bf16* p = a.q + ((int64_t)it.b * a.T + (live ? i : 0)) * a.q_stride +
                         (it.h * a.G + (live ? row % a.G : 0)) * D + t * (D / 4);
         uint32_t h[D / 8];
-        sc[k] = a.scale_log2 * ka_load_q<D / 4>(p, live, h);
+        sc[k] = fmaxf(a.scale_log2 * ka_load_q<D / 4>(p, live, h, a.negate), 1e-37f);  // never 0: 0 x -inf
 #pragma unroll
         for (int s = 0; s < 2 * KW; ++s) {
           qa[s][k] = h[2 * s];
@@ -361,7 +364,7 @@ __global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
       float o[NV][4];
 #pragma unroll
       for (int i = 0; i < NV; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      float m[2] = {-INFINITY, -INFINITY}, l[4] = {0.f, 0.f, 0.f, 0.f};  // l: sums of rows g and g + 8 in [0] and [2]
       // cache rows that every row of the tile sees
       const int all_hi = it.x.pos + it.x.t0;
       const int all_lo = a.window > 0 ? it.x.pos + it.x.t1 - a.window + 1 : 0;
@@ -369,61 +372,68 @@ __global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
       for (int c = it.c0; c < it.c1; ++c, ++n) {
         const uint32_t s = n % kKaStages;
         if (!bad) bad = !__all_sync(0xffffffffu, tc_wait_err(&full[s], (n / kKaStages) & 1, abort, &g_kv4_error));
-        const int key0 = it.first_key(c) + warp * 16;
-        if (!bad && (present[s] >> warp & 1u)) {
+        const int key0 = it.first_key(c) + warp * kKaKeys;
+        // 16-row pieces of this warp's rows that were copied
+        const uint32_t here = bad ? 0u : (present[s] >> (warp * kKaPieces)) & ((1u << kKaPieces) - 1u);
+        if (here) {
           const unsigned char* st = ring + s * S::kStage;
-          const bool masked = key0 + 15 > all_hi || (key0 < all_lo && key0 + 15 >= a.sinks);
-          float sa[2][4];
+          const bool masked = here != (1u << kKaPieces) - 1u || key0 + kKaKeys - 1 > all_hi ||
+                              (key0 < all_lo && key0 + kKaKeys > a.sinks);
+          auto see = [&](int e, int p) {  // cache row key0 + e from position p
+            const int key = key0 + e;
+            return key <= p && (a.window == 0 || key > p - a.window || key < a.sinks) && (here >> (e / 16) & 1u);
+          };
+          // ---- S = Q K^T ----
+          float sa[kKaKeys / 8][4];
+          uint32_t kw[kKaKeys / 8][KW], kf[kKaKeys / 8][2];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int r = warp * 16 + j * 8 + g;
-            uint32_t w[KW], sg[2];
+          for (int j = 0; j < kKaKeys / 8; ++j) {
+            const int r = warp * kKaKeys + j * 8 + g;
             if constexpr (D == 128) {
               const uint4 v = *reinterpret_cast<const uint4*>(st + r * (D / 2) + t * 16);
-              w[0] = v.x;
-              w[1] = v.y;
-              w[2] = v.z;
-              w[3] = v.w;
+              kw[j][0] = v.x;
+              kw[j][1] = v.y;
+              kw[j][2] = v.z;
+              kw[j][3] = v.w;
               const uint32_t x = e4m3x2_to_h2(*reinterpret_cast<const uint16_t*>(st + kv4_off_ks(kKaChunk, D) + r * 8 + t * 2));
-              sg[0] = __byte_perm(x, 0, 0x1010);
-              sg[1] = __byte_perm(x, 0, 0x3232);
+              kf[j][0] = __byte_perm(x, 0, 0x1010);
+              kf[j][1] = __byte_perm(x, 0, 0x3232);
             } else {
               const uint2 v = *reinterpret_cast<const uint2*>(st + r * (D / 2) + t * 8);
-              w[0] = v.x;
-              w[1] = v.y;
+              kw[j][0] = v.x;
+              kw[j][1] = v.y;
               const uint32_t x = st[kv4_off_ks(kKaChunk, D) + r * 4 + t];
-              sg[0] = sg[1] = e4m3x2_to_h2(x | (x << 8));
+              kf[j][0] = kf[j][1] = e4m3x2_to_h2(x | (x << 8));
             }
             sa[j][0] = sa[j][1] = sa[j][2] = sa[j][3] = 0.f;
+          }
 #pragma unroll
-            for (int k = 0; k < KW; ++k) {
+          for (int k = 0; k < KW; ++k)
+#pragma unroll
+            for (int j = 0; j < kKaKeys / 8; ++j) {
               uint32_t h[4];
-              e2m1x8_to_h2(w[k], h);
-              const uint32_t f = sg[k * 2 / KW];
+              e2m1x8_to_h2(kw[j][k], h);
+              const uint32_t f = kf[j][k * 2 / KW];
               ka_mma(sa[j], qa[2 * k], hmul2_u(h[0], f), hmul2_u(h[1], f));
               ka_mma(sa[j], qa[2 * k + 1], hmul2_u(h[2], f), hmul2_u(h[3], f));
             }
+          if (masked) {
+#pragma unroll
+            for (int j = 0; j < kKaKeys / 8; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (!see(j * 8 + 2 * t + (e & 1), rowpos[e >> 1])) sa[j][e] = -INFINITY;
           }
-          // scores in units of log2, masked; the running reference
-          float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float v = sa[j][e] * sc[e >> 1];
-              if (masked) {
-                const int key = key0 + j * 8 + 2 * t + (e & 1), p = rowpos[e >> 1];
-                const bool see = key <= p && (a.window == 0 || key > p - a.window || key < a.sinks);
-                v = see ? v : -INFINITY;
-              }
-              sa[j][e] = v;
-              top[e >> 1] = fmaxf(top[e >> 1], v);
-            }
+          // ---- running reference, weights ----
           bool move = false;
+          float top[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
+            top[k] = fmaxf(sa[0][2 * k], sa[0][2 * k + 1]);
+#pragma unroll
+            for (int j = 1; j < kKaKeys / 8; ++j) top[k] = fmaxf(top[k], fmaxf(sa[j][2 * k], sa[j][2 * k + 1]));
             top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
-            top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
+            top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2)) * sc[k];
             move |= top[k] > m[k] + kKaLazy;
           }
           if (__any_sync(0xffffffffu, move)) {
@@ -432,7 +442,7 @@ __global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
               const float to = top[k] > m[k] + kKaLazy ? top[k] : m[k];
               const float f = m[k] == -INFINITY ? 0.f : ka_exp2(m[k] - to);
               m[k] = to;
-              l[k] *= f;
+              l[2 * k] *= f;
 #pragma unroll
               for (int i = 0; i < NV; ++i) {
                 o[i][2 * k] *= f;
@@ -440,78 +450,68 @@ __global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
               }
             }
           }
-          const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0] - kKaOff, m[1] == -INFINITY ? 0.f : m[1] - kKaOff};
-          uint32_t pa[4];
+          const float ref[2] = {m[0] == -INFINITY ? 0.f : kKaOff - m[0], m[1] == -INFINITY ? 0.f : kKaOff - m[1]};
+          uint32_t pa[kKaPieces][4];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
+          for (int j = 0; j < kKaKeys / 8; ++j) {
             float p[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              p[e] = ka_exp2(sa[j][e] - ref[e >> 1]);
-              l[e >> 1] += p[e];
-            }
-            pa[2 * j] = ka_h2(p[0], p[1]);
-            pa[2 * j + 1] = ka_h2(p[2], p[3]);
+            for (int e = 0; e < 4; ++e) p[e] = ka_exp2(__fmaf_rn(sa[j][e], sc[e >> 1], ref[e >> 1]));
+            pa[j / 2][j % 2 * 2] = ka_h2(p[0], p[1]);
+            pa[j / 2][j % 2 * 2 + 1] = ka_h2(p[2], p[3]);
           }
-          // V: this lane's rows 2t, 2t + 1 of both 8-row halves, column g
-          uint32_t sv[4];
-          const unsigned char* vs = st + kv4_off_vs(kKaChunk, D);
-          const unsigned char* vc = st + kv4_off_v(kKaChunk, D);
+          // ---- O += P V, and the weights' sum as one more column of ones ----
+          const unsigned char* vs = st + kv4_off_vs(kKaChunk, D) + warp * kKaKeys * (D / 16);
+          const unsigned char* vc = st + kv4_off_v(kKaChunk, D) + warp * kKaKeys * (D / 2);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            sv[k] = vs[(warp * 16 + (k >> 1) * 8 + 2 * t + (k & 1)) * (D / 16) + g * NV / 16];
-          if (masked) {
-            // a weight of 0 does not silence a NaN: rows that some of the tile must not see
-            // enter without their NaN scales, which are put into the rows that do see them
-            bool odd = false;
+          for (int u = 0; u < kKaPieces; ++u) {
+            // this lane's rows 2t, 2t + 1 of both 8-row halves, column g
+            uint32_t sv[4], w[4][VW];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              odd |= ka_nan_scale(sv[k]);
-              if (ka_nan_scale(sv[k])) sv[k] = 0;
-            }
-            if (__any_sync(0xffffffffu, odd)) {
-              for (int e = 0; e < 16; ++e) {
-                const int key = key0 + e;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  const int p = rowpos[k];
-                  const bool see = key <= p && (a.window == 0 || key > p - a.window || key < a.sinks);
-#pragma unroll
-                  for (int col = 0; col < 2; ++col)
-                    if (see && ka_nan_scale(vs[(warp * 16 + e) * (D / 16) + (2 * t + col) * NV / 16]))
-#pragma unroll
-                      for (int i = 0; i < NV; ++i) o[i][2 * k + col] = NAN;
-                }
-              }
-            }
-          }
-          const uint32_t f0 = e4m3x2_to_h2(sv[0] | (sv[1] << 8)), f1 = e4m3x2_to_h2(sv[2] | (sv[3] << 8));
-          uint32_t w[4][VW];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const unsigned char* p = vc + (warp * 16 + (k >> 1) * 8 + 2 * t + (k & 1)) * (D / 2) + g * (NV / 2);
-            if constexpr (D == 128) {
-              const uint2 v = *reinterpret_cast<const uint2*>(p);
-              w[k][0] = v.x;
-              w[k][1] = v.y;
-            } else {
-              w[k][0] = *reinterpret_cast<const uint32_t*>(p);
-            }
-          }
-#pragma unroll
-          for (int x = 0; x < VW; ++x) {
-#pragma unroll
-            for (int par = 0; par < 2; ++par) {  // even and odd dimensions of the word
-              uint32_t h0[4], h1[4];
-              if (par == 0) {
-                e2m1x8_to_h2((w[0][x] & 0x0f0f0f0fu) | ((w[1][x] << 4) & 0xf0f0f0f0u), h0);
-                e2m1x8_to_h2((w[2][x] & 0x0f0f0f0fu) | ((w[3][x] << 4) & 0xf0f0f0f0u), h1);
+              const int r = u * 16 + (k >> 1) * 8 + 2 * t + (k & 1);
+              sv[k] = vs[r * (D / 16) + g * NV / 16];
+              if constexpr (D == 128) {
+                const uint2 v = *reinterpret_cast<const uint2*>(vc + r * (D / 2) + g * (NV / 2));
+                w[k][0] = v.x;
+                w[k][1] = v.y;
               } else {
-                e2m1x8_to_h2(((w[0][x] >> 4) & 0x0f0f0f0fu) | (w[1][x] & 0xf0f0f0f0u), h0);
-                e2m1x8_to_h2(((w[2][x] >> 4) & 0x0f0f0f0fu) | (w[3][x] & 0xf0f0f0f0u), h1);
+                w[k][0] = *reinterpret_cast<const uint32_t*>(vc + r * (D / 2) + g * (NV / 2));
               }
+            }
+            if (masked) {
+              // a weight of 0 does not silence a NaN: rows that some of the tile must not see
+              // enter without their NaN scales, which are put into the rows that do see them
+              bool odd = false;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) ka_mma(o[8 * x + 2 * k + par], pa, hmul2_u(h0[k], f0), hmul2_u(h1[k], f1));
+              for (int k = 0; k < 4; ++k) {
+                odd |= ka_nan_scale(sv[k]);
+                if (ka_nan_scale(sv[k])) sv[k] = 0;
+              }
+              if (__any_sync(0xffffffffu, odd)) {
+                for (int e = u * 16; e < u * 16 + 16; ++e)
+#pragma unroll
+                  for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int col = 0; col < 2; ++col)
+                      if (see(e, rowpos[k]) && ka_nan_scale(vs[e * (D / 16) + (2 * t + col) * NV / 16]))
+#pragma unroll
+                        for (int i = 0; i < NV; ++i) o[i][2 * k + col] = NAN;
+              }
+            }
+            const uint32_t f0 = e4m3x2_to_h2(sv[0] | (sv[1] << 8)), f1 = e4m3x2_to_h2(sv[2] | (sv[3] << 8));
+            ka_mma(l, pa[u], 0x3c003c00u, 0x3c003c00u);
+#pragma unroll
+            for (int x = 0; x < VW; ++x) {
+              uint32_t h0[4], h1[4];  // even dimensions of the word, then odd ones
+              e2m1x8_to_h2((w[0][x] & 0x0f0f0f0fu) | ((w[1][x] << 4) & 0xf0f0f0f0u), h0);
+              e2m1x8_to_h2((w[2][x] & 0x0f0f0f0fu) | ((w[3][x] << 4) & 0xf0f0f0f0u), h1);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) ka_mma(o[8 * x + 2 * k], pa[u], hmul2_u(h0[k], f0), hmul2_u(h1[k], f1));
+              e2m1x8_to_h2(((w[0][x] >> 4) & 0x0f0f0f0fu) | (w[1][x] & 0xf0f0f0f0u), h0);
+              e2m1x8_to_h2(((w[2][x] >> 4) & 0x0f0f0f0fu) | (w[3][x] & 0xf0f0f0f0u), h1);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) ka_mma(o[8 * x + 2 * k + 1], pa[u], hmul2_u(h0[k], f0), hmul2_u(h1[k], f1));
             }
           }
         }
@@ -522,12 +522,10 @@ __global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
       // ---- join the four warps ----
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
-        l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
         const int r = g + 8 * k;
         if (t == 0) {
           join_m[warp * kKaRows + r] = m[k];
-          join_l[warp * kKaRows + r] = l[k];
+          join_l[warp * kKaRows + r] = l[2 * k];
         }
         float* row = join + (warp * kKaRows + r) * S::kPad;
 #pragma unroll
@@ -600,28 +598,48 @@ __global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
           ka_sync();
           if (!flags[1]) break;
           __threadfence();
-          float* wgt = join;  // [members][16]
-          if (tid < kKaRows) {
-            float top = -INFINITY, sum = 0.f;
-            for (int p = 0; p < members; ++p)
-              top = fmaxf(top, __ldcg(a.parts + slot_of((lead + p) * span) * S::kRecord + kKaRows * D + tid));
-            for (int p = 0; p < members; ++p) {
-              const float* r = a.parts + slot_of((lead + p) * span) * S::kRecord + kKaRows * D + tid;
-              const float mp = __ldcg(r), f = mp == -INFINITY ? 0.f : ka_exp2(mp - top);
-              wgt[p * kKaRows + tid] = f;
-              sum += __ldcg(r + kKaRows) * f;
+          float* wgt = join;                                              // [members][16]
+          float** recs = reinterpret_cast<float**>(join + kKaFan * kKaRows);  // [members]
+          if (tid < members) recs[tid] = a.parts + slot_of((lead + tid) * span) * S::kRecord;
+          ka_sync();
+          for (int e = tid; e < members * kKaRows; e += kKaWarps * 32)
+            wgt[e] = __ldcg(recs[e / kKaRows] + kKaRows * D + e % kKaRows);
+          float lp[kKaFan * kKaRows / (kKaWarps * 32)];
+#pragma unroll
+          for (int k = 0; k < kKaFan * kKaRows / (kKaWarps * 32); ++k) {
+            const int e = tid + k * kKaWarps * 32;
+            lp[k] = e < members * kKaRows ? __ldcg(recs[e / kKaRows] + kKaRows * D + kKaRows + e % kKaRows) : 0.f;
+          }
+          ka_sync();
+          float top = -INFINITY;  // of row tid % 16
+          for (int p = 0; p < members; ++p) top = fmaxf(top, wgt[p * kKaRows + tid % kKaRows]);
+          ka_sync();
+          float* sums = join + kKaFan * kKaRows * 2;  // [members][16]
+#pragma unroll
+          for (int k = 0; k < kKaFan * kKaRows / (kKaWarps * 32); ++k) {
+            const int e = tid + k * kKaWarps * 32;
+            if (e < members * kKaRows) {
+              const float f = wgt[e] == -INFINITY ? 0.f : ka_exp2(wgt[e] - top);
+              wgt[e] = f;
+              sums[e] = lp[k] * f;
             }
+          }
+          ka_sync();
+          if (tid < kKaRows) {
+            float sum = 0.f;
+            for (int p = 0; p < members; ++p) sum += sums[p * kKaRows + tid];
             join_m[tid] = top;
             join_l[tid] = sum;
           }
           ka_sync();
-          float* dst = a.parts + slot_of(lead * span) * S::kRecord;
+          float* dst = recs[0];
           for (int e = tid; e < kKaRows * D / 4; e += kKaWarps * 32) {
             const int r = e / (D / 4), d = e % (D / 4) * 4;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-            for (int p = 0; p < members; ++p) {
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(a.parts + slot_of((lead + p) * span) * S::kRecord + r * D + d));
+#pragma unroll
+            for (int p = 0; p < kKaFan; ++p) {
+              if (p >= members) break;
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(recs[p] + r * D + d));
               const float f = wgt[p * kKaRows + r];
               acc.x += v.x * f;
               acc.y += v.y * f;
@@ -702,6 +720,7 @@ extern "C" int jsx_kv4_attn(const void* q, int64_t q_stride, const void* pool, i
                   q_stride >= (int64_t)nq * head_dim && out_stride >= (int64_t)nq * head_dim,
               "q and out must be 16-byte aligned, with token strides of at least nq * head_dim in multiples of 8");
   JSX_REQUIRE(window >= 0 && sinks >= 0, "window=%d sinks=%d", window, sinks);
+  JSX_REQUIRE(fabsf(scale) <= 1e30f, "scale %g", (double)scale);
   size_t need = 0;
   const int st = jsx_kv4_attn_workspace_size(B, T, nq, nkv, head_dim, &need);
   if (st) return st;
@@ -728,7 +747,8 @@ extern "C" int jsx_kv4_attn(const void* q, int64_t q_stride, const void* pool, i
   a.pt = page_tokens;
   a.window = window < (1 << 30) ? window : 1 << 30;  // (positions are below 2^30)
   a.sinks = sinks;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.negate = scale < 0.f ? 0x80000000u : 0u;
+  a.scale_log2 = fabsf(scale) * 1.4426950408889634f;
   a.listed = (int64_t)B * a.tiles <= kKaListMax;
   const int64_t items = (int64_t)B * nkv * a.tiles;
   const int64_t units = a.listed ? items * (((int64_t)table_slots * page_tokens + kKaChunk - 1) / kKaChunk) : items;
