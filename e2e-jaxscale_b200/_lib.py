@@ -122,7 +122,7 @@ lib = _load()
 def call(name: str, *args) -> None:
     """Call a jsx_* entry point and raise JsxError on a non-zero status."""
     st = getattr(lib, name)(*args)
-    if st != JSX_OK:
+    if st:
         raise JsxError(st, name, (lib.jsx_last_error() or b"").decode(errors="replace"))
 
 

@@ -13,7 +13,7 @@
 // workspace, and the last CTA of each group of 16 to arrive joins the group, in part
 // order: the result does not depend on who is last.
 //
-// Inside a CTA one warp copies a chunk's codes and scales into a ring of shared-memory
+// Inside a CTA a chunk's codes and scales are copied into a ring of shared-memory
 // stages (cp.async.bulk, 18 KB per stage at head_dim 128) and four warps take 32 of its
 // 128 cache rows each, with their own running maximum and sum.  S = Q K^T and O += P V run on
 // mma.sync m16n8k16 f16: a stored value (at most 6 significant bits) is exact in f16,
@@ -38,11 +38,12 @@ constexpr int kKaChunk = 128;   // cache rows per stage
 constexpr int kKaWarps = 4;     // computing warps, 32 cache rows of a chunk each
 constexpr int kKaKeys = kKaChunk / kKaWarps;
 constexpr int kKaPieces = kKaKeys / 16;
-constexpr int kKaThreads = (kKaWarps + 1) * 32;
+constexpr int kKaThreads = (kKaWarps + 1) * 32;  // and one that copies
+constexpr int kKaPerSm = 3;     // CTAs per SM
 constexpr int kKaStages = 3;
 constexpr int kKaFan = 16;      // parts joined at once
 constexpr int kKaLevels = 3;    // 16^3 parts of an item at most
-constexpr int kKaListMax = 1024;  // (sequence, row tile) pairs up to which the chunk list is cut into ranges
+constexpr int kKaListMax = 512;   // (sequence, row tile) pairs up to which the chunk list is cut into ranges
 constexpr float kKaOff = 10.f;  // weights are 2^(s - m + 10): f16 holds them down to 2^-34 of the largest
 constexpr float kKaLazy = 4.f;  // the reference m moves when the maximum exceeds it by this much
 
@@ -65,7 +66,8 @@ struct KaArgs {
   const int32_t* n_tokens;
   float* parts;       // [2 x CTAs] records
   uint32_t* arrived;  // [kKaLevels][2 x CTAs], zero between calls
-  int num_pages, slots, B, T, nkv, G, tiles, pt, window, sinks;
+  int num_pages, slots, B, T, nkv, G, tiles, pt, pt_log, window, sinks;
+  uint32_t per_g;  // 2^32 / G rounded up: x / G = umulhi(x, per_g) for x G < 2^32 (G > 1)
   int listed;  // chunk list cut into ranges; else whole items per CTA
   uint32_t negate;   // 0x80000000 when the scale is negative
   float scale_log2;  // its magnitude x log2(e)
@@ -74,11 +76,10 @@ struct KaArgs {
 template <int D>
 struct KaShape {
   static constexpr int kStage = kv4_block_bytes(kKaChunk, D);
-  static constexpr int kRecord = kKaRows * D + 2 * kKaRows;  // floats
-  static constexpr int kPad = D + 16;                        // row stride of the joining buffer, floats
-  static constexpr int kJoin = kKaWarps * kKaRows * (kPad + 2) * 4;
-  static constexpr size_t kSmem = (size_t)kKaStages * kStage + kJoin + (kKaListMax + 1) * 8 + 256;
+  static constexpr int kRecord = kKaRows * D + 2 * kKaRows;  // floats: output, maxima, sums
 };
+
+__device__ __forceinline__ int ka_div_g(const KaArgs& a, int x) { return a.G == 1 ? x : (int)__umulhi((uint32_t)x, a.per_g); }
 
 // Rows of one (sequence, row tile): tokens t0..t1, cache rows below `hi`, chunks.
 struct KaTile {
@@ -89,8 +90,8 @@ __device__ __forceinline__ KaTile ka_tile(const KaArgs& a, int b, int tile) {
   KaTile x;
   x.pos = min(a.positions[b], 1 << 30);
   x.used = a.n_tokens ? min(max(a.n_tokens[b], 0), a.T) : a.T;
-  x.t0 = tile * kKaRows / a.G;
-  x.t1 = min(min(tile * kKaRows + kKaRows - 1, a.G * a.T - 1) / a.G, x.used - 1);
+  x.t0 = ka_div_g(a, tile * kKaRows);
+  x.t1 = min(ka_div_g(a, min(tile * kKaRows + kKaRows, a.G * a.T) - 1), x.used - 1);
   x.hi = min(max(x.pos + x.t1 + 1, 0), a.slots * a.pt);
   x.n = x.lo_chunk = x.sink_chunks = 0;
   if (x.t0 > x.t1 || x.hi == 0) return x;
@@ -102,83 +103,116 @@ __device__ __forceinline__ KaTile ka_tile(const KaArgs& a, int b, int tile) {
   return x;
 }
 
-// The items of one CTA, in order, with the chunks [c0, c1) of each that are its own.
-struct KaWalk {
-  const KaArgs& a;
-  const long long* cum;  // [B + 1] chunks before each sequence
-  long long w, w1, total, ctas;  // ctas: CTAs with a range (at least one chunk each)
+// A place in the list: an item, with the chunks [c0, c1) of it that are this CTA's.  Kept
+// in shared memory, one for the copying warp and one for the computing ones.
+struct KaPos {
+  int live;
   int b, h, tile, c0, c1;
-  long long item;
+  int w, w1;         // place and end in the list
+  int share, extra;  // how the list is cut
   KaTile x;
-  __device__ KaWalk(const KaArgs& args, const long long* sums) : a(args), cum(sums) {}
-  __device__ void locate() {
-    h = (int)(item / a.tiles % a.nkv);
-    b = (int)(item / a.tiles / a.nkv);
-    tile = (int)(item % a.tiles);
-    x = ka_tile(a, b, tile);
-    c0 = 0;
-    c1 = x.n;
-  }
-  __device__ bool begin() {
-    if (!a.listed) {
-      item = blockIdx.x;
-      if (item >= (long long)a.B * a.nkv * a.tiles) return false;
-      locate();
-      return true;
-    }
-    total = cum[a.B];
-    ctas = min((long long)gridDim.x, total);
-    if (blockIdx.x >= ctas) return false;
-    w = total * blockIdx.x / ctas;
-    w1 = total * (blockIdx.x + 1) / ctas;
-    int lo = 0, hi = a.B;  // the last sequence whose chunks begin at or before w
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (cum[mid] <= w) lo = mid;
-      else hi = mid;
-    }
-    b = lo;
-    long long off = w - cum[b];
-    const long long per = (cum[b + 1] - cum[b]) / a.nkv;
-    h = (int)(off / per);
-    off -= h * per;
-    for (tile = 0;; ++tile) {
-      x = ka_tile(a, b, tile);
-      if (off < x.n) break;
-      off -= x.n;
-    }
-    c0 = (int)off;
-    c1 = (int)min((long long)x.n, off + (w1 - w));
-    return true;
-  }
-  __device__ bool next() {
-    if (!a.listed) {
-      item += gridDim.x;
-      if (item >= (long long)a.B * a.nkv * a.tiles) return false;
-      locate();
-      return true;
-    }
-    w += c1 - c0;
-    if (w >= w1) return false;
-    do {
-      if (++tile == a.tiles) {
-        tile = 0;
-        if (++h == a.nkv) {
-          h = 0;
-          do ++b;
-          while (cum[b + 1] == cum[b]);
-        }
-      }
-      x = ka_tile(a, b, tile);
-    } while (x.n == 0);
-    c0 = 0;
-    c1 = (int)min((long long)x.n, w1 - w);
-    return true;
-  }
-  __device__ int first_key(int c) const {
-    return (c < x.sink_chunks ? c : x.lo_chunk + c - x.sink_chunks) * kKaChunk;
-  }
 };
+
+// The list is cut into ranges of `share` + 1 places (the first `extra` CTAs) and `share`:
+// where CTA `cta`'s range begins, and the CTA whose range holds place u.
+__device__ __forceinline__ int ka_range(const KaPos& p, int cta) { return cta * p.share + min(cta, p.extra); }
+__device__ __forceinline__ int ka_owner(const KaPos& p, int u) {
+  const uint32_t big = (uint32_t)p.share + 1u, edge = (uint32_t)p.extra * big;
+  return (uint32_t)u < edge ? (uint32_t)u / big : p.extra + ((uint32_t)u - edge) / (uint32_t)p.share;
+}
+
+// The place after *p; cum[b]: chunks before sequence b.  Called by one thread: out of
+// line, so that its code is there once.
+__device__ __noinline__ void ka_next(const KaArgs& a, const int* cum, KaPos* p) {
+  KaPos q = *p;
+  if (!a.listed) {
+    q.w += gridDim.x;
+    q.live = q.w < a.B * a.nkv * a.tiles;
+    if (q.live) {
+      q.tile = q.w % a.tiles;
+      q.h = q.w / a.tiles % a.nkv;
+      q.b = q.w / a.tiles / a.nkv;
+      q.x = ka_tile(a, q.b, q.tile);
+    }
+  } else {
+    q.w += q.c1 - q.c0;
+    q.live = q.w < q.w1;
+    if (q.live) do {
+        if (++q.tile == a.tiles) {
+          q.tile = 0;
+          if (++q.h == a.nkv) {
+            q.h = 0;
+            do ++q.b;
+            while (cum[q.b + 1] == cum[q.b]);
+          }
+        }
+        q.x = ka_tile(a, q.b, q.tile);
+      } while (q.x.n == 0);
+  }
+  q.c0 = 0;
+  q.c1 = a.listed ? min(q.x.n, q.w1 - q.w) : q.x.n;
+  *p = q;
+}
+
+// The CTA's first place, by one warp; in the listed form cum is filled on the way.
+__device__ __forceinline__ KaPos ka_first(const KaArgs& a, int* cum, int lane) {
+  KaPos q;
+  if (!a.listed) {
+    q.w = blockIdx.x;
+    q.live = 1;
+    q.tile = q.w % a.tiles;
+    q.h = q.w / a.tiles % a.nkv;
+    q.b = q.w / a.tiles / a.nkv;
+    q.x = ka_tile(a, q.b, q.tile);
+    q.c0 = 0;
+    q.c1 = q.x.n;
+    q.w1 = q.share = q.extra = 0;
+    return q;
+  }
+  uint32_t total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int b = b0 + lane;
+    int n = 0;
+    if (b < a.B)
+      for (int t = 0; t < a.tiles; ++t) n += ka_tile(a, b, t).n;
+    n *= a.nkv;
+    int v = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += y;
+    }
+    if (b < a.B) cum[b + 1] = total + v;
+    total += __shfl_sync(0xffffffffu, v, 31);
+  }
+  if (lane == 0) cum[0] = 0;
+  __syncwarp();
+  // CTAs with a range have a chunk at least
+  q.share = total <= gridDim.x ? 1 : total / gridDim.x;
+  q.extra = total <= gridDim.x ? 0 : total - q.share * gridDim.x;
+  q.live = blockIdx.x < total;
+  q.w = ka_range(q, blockIdx.x);
+  q.w1 = ka_range(q, blockIdx.x + 1);
+  q.b = q.h = q.tile = q.c0 = q.c1 = 0;
+  if (!q.live) return q;
+  int n = 0;  // sequences whose chunks begin at or before w: the last of them is it
+  for (int b0 = 0; b0 < a.B; b0 += 32) n += __popc(__ballot_sync(0xffffffffu, b0 + lane < a.B && cum[b0 + lane] <= q.w));
+  q.b = n - 1;
+  int off = q.w - cum[q.b], per = 0;
+  for (int t = 0; t < a.tiles; ++t) per += ka_tile(a, q.b, t).n;
+  while (off >= per) {
+    off -= per;
+    ++q.h;
+  }
+  for (;; ++q.tile) {
+    q.x = ka_tile(a, q.b, q.tile);
+    if (off < q.x.n) break;
+    off -= q.x.n;
+  }
+  q.c0 = off;
+  q.c1 = min(q.x.n, off + q.w1 - q.w);
+  return q;
+}
 
 __device__ __forceinline__ void ka_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(s_u32(dst)),
@@ -186,8 +220,7 @@ __device__ __forceinline__ void ka_copy(void* dst, const void* src, uint32_t byt
                : "memory");
 }
 __device__ __forceinline__ void ka_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -200,7 +233,7 @@ __device__ __forceinline__ uint32_t ka_h2(float lo, float hi) {
   __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&h);
 }
-__device__ __forceinline__ void ka_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void ka_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }  // the computing warps
 __device__ __forceinline__ bool ka_nan_scale(uint32_t s) { return (s & 0x7fu) == 0x7fu; }
 
 // One row's D / 4 values of q at `p` as f16 pairs, scaled by the power of two that brings
@@ -230,33 +263,29 @@ __device__ __forceinline__ float ka_load_q(const bf16* p, bool live, uint32_t (&
   return f == 254 ? 0x1p-127f : __uint_as_float((uint32_t)(254 - f) << 23);
 }
 
-// This thread's part of a row tile's result: 4 values of row r from dimension d on.
-__device__ __forceinline__ void ka_store(const KaArgs& a, const KaWalk& it, int D, int r, int d, float4 o, float l) {
-  const int row = it.tile * kKaRows + r;
-  if (row >= a.G * a.T) return;
-  const int i = row / a.G, g = row % a.G;
-  const float f = l == 0.f || i >= it.x.used ? 0.f : 1.f / l;
-  uint2 v = make_uint2(pack2(o.x * f, o.y * f), pack2(o.z * f, o.w * f));
-  if (i >= it.x.used) v = make_uint2(0, 0);
-  *reinterpret_cast<uint2*>(a.out + ((int64_t)it.b * a.T + i) * a.out_stride + (it.h * a.G + g) * D + d) = v;
+// Four values of a row's result; `l` is the weights' sum.
+__device__ __forceinline__ void ka_store(bf16* out, float4 o, float l) {
+  const float f = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack2(o.x * f, o.y * f), pack2(o.z * f, o.w * f));
 }
 
 template <int D>
-__global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
+__global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_constant__ KaArgs a) {
   using S = KaShape<D>;
   constexpr int KW = D / 32;      // words of codes per lane and K row
   constexpr int NV = D / 8;       // n tiles of O = dimensions per column
   constexpr int VW = D / 64;      // words of codes per lane and V row
-  extern __shared__ __align__(128) unsigned char smem[];
-  unsigned char* ring = smem;
-  float* join = reinterpret_cast<float*>(smem + kKaStages * S::kStage);  // [warps][16][kPad], then m and l
-  float* join_m = join + kKaWarps * kKaRows * S::kPad;                   // [warps][16]
-  float* join_l = join_m + kKaWarps * kKaRows;
-  long long* cum = reinterpret_cast<long long*>(smem + kKaStages * S::kStage + S::kJoin);
-  uint64_t* full = reinterpret_cast<uint64_t*>(cum + kKaListMax + 1);
-  uint64_t* empty = full + kKaStages;
-  uint32_t* present = reinterpret_cast<uint32_t*>(empty + kKaStages);  // per stage: 16-row pieces that were copied
-  uint32_t* flags = present + kKaStages;                               // [0] a wait gave up, [1] last to arrive
+  extern __shared__ __align__(128) unsigned char ring[];
+  __shared__ __align__(16) float join[2 * kKaRows * D];  // two warps' outputs; before that q as MMA operands [D / 16][32 lanes]
+  __shared__ float join_m[2 * kKaRows], join_l[2 * kKaRows];
+  __shared__ int cum[kKaListMax + 1];
+  __shared__ KaPos place[2];
+  __shared__ uint64_t full[kKaStages], empty[kKaStages];
+  __shared__ uint32_t present[kKaStages];  // pages of the stage that were copied
+  __shared__ uint32_t flags[2];            // [0] a wait gave up, [1] last to arrive
+  __shared__ int row_token[kKaRows], row_head[kKaRows];
+  __shared__ float* recs[kKaFan];
+  uint4* qfrag = reinterpret_cast<uint4*>(join);
   volatile uint32_t* abort = flags;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
@@ -269,70 +298,51 @@ __global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   pdl_wait();
-  if (a.listed && warp == 0) {
-    // chunks before each sequence
-    long long run = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-      const int b = b0 + lane;
-      long long n = 0;
-      if (b < a.B)
-        for (int t = 0; t < a.tiles; ++t) n += ka_tile(a, b, t).n;
-      n *= a.nkv;
-      long long v = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += y;
-      }
-      if (b < a.B) cum[b + 1] = run + v;
-      run += __shfl_sync(0xffffffffu, v, 31);
-    }
-    if (lane == 0) cum[0] = 0;
+  if (warp == kKaWarps) {
+    const KaPos q = ka_first(a, cum, lane);
+    if (lane == 0) place[0] = place[1] = q;
   }
   __syncthreads();
+  const uint32_t block = kv4_block_bytes(a.pt, D);
 
   if (warp == kKaWarps) {
-    // ---- copies: lane = (page of the chunk, array) ----
-    KaWalk it(a, cum);
-    const int run = min(a.pt, kKaChunk), pages = kKaChunk / run;
-    const int j = lane >> 2, arr = lane & 3;
-    uint32_t n = 0;
-    if (it.begin()) do {
-        for (int c = it.c0; c < it.c1; ++c, ++n) {
-          const uint32_t s = n % kKaStages;
-          const int key = it.first_key(c) + j * run, slot = key / a.pt;
-          const int lim = c < it.x.sink_chunks ? min(a.sinks, it.x.hi) : it.x.hi;
-          int rows = j < pages ? min(max((lim - key + 15) & ~15, 0), run) : 0;
-          int page = -1;
-          if (rows > 0 && slot < a.slots) page = a.table[(int64_t)it.b * a.slots + slot];
-          if (page < 0 || page >= a.num_pages) rows = 0;
-          const uint32_t bytes = rows * (arr < 2 ? D / 2 : D / 16);
-          const uint32_t sum = __reduce_add_sync(0xffffffffu, bytes);
-          const uint32_t bits = __reduce_or_sync(0xffffffffu, arr == 0 ? ((1u << (rows / 16)) - 1u) << (j * run / 16) : 0u);
-          if (n >= kKaStages &&
-              !__all_sync(0xffffffffu, tc_wait_err(&empty[s], (n / kKaStages - 1) & 1, abort, &g_kv4_error)))
-            goto drained;
-          if (lane == 0) {
-            present[s] = bits;
-            tc_expect_tx(&full[s], sum);
-          }
-          __syncwarp();
-          if (bytes) {
-            const uint8_t* src = a.pool + ((int64_t)page * a.nkv + it.h) * kv4_block_bytes(a.pt, D);
-            const int row = key - slot * a.pt;
-            unsigned char* dst = ring + s * S::kStage;
-            if (arr < 2)
-              ka_copy(dst + arr * kv4_off_v(kKaChunk, D) + j * run * (D / 2),
-                      src + arr * kv4_off_v(a.pt, D) + row * (D / 2), bytes, &full[s]);
-            else
-              ka_copy(dst + (arr == 2 ? kv4_off_ks(kKaChunk, D) : kv4_off_vs(kKaChunk, D)) + j * run * (D / 16),
-                      src + (arr == 2 ? kv4_off_ks(a.pt, D) : kv4_off_vs(a.pt, D)) + row * (D / 16), bytes, &full[s]);
-          }
+    // ---- copies: a lane per page of the chunk, a whole page's block at once ----
+    KaPos& p = place[1];
+    const int pages = kKaChunk >> a.pt_log;
+    uint32_t f = 0;
+    while (p.live) {
+      const int c0 = p.c0, c1 = p.c1, lo_chunk = p.x.lo_chunk, sink_chunks = p.x.sink_chunks, hi = p.x.hi;
+      const int sinks = min(a.sinks, hi);
+      const int32_t* row = a.table + (int64_t)p.b * a.slots;
+      const int64_t head = p.h;
+      auto look_up = [&](int c) {
+        const int chunk = c < sink_chunks ? c : lo_chunk + c - sink_chunks;
+        const int slot = chunk * pages + lane;
+        return lane < pages && (slot << a.pt_log) < (c < sink_chunks ? sinks : hi) && slot < a.slots ? row[slot] : -1;
+      };
+      int soon = c0 < c1 ? look_up(c0) : -1;  // pages are looked up a chunk ahead
+      for (int c = c0; c < c1; ++c, ++f) {
+        const uint32_t s = f % kKaStages;
+        const int page = soon;
+        if (c + 1 < c1) soon = look_up(c + 1);
+        if (f >= kKaStages && !__all_sync(0xffffffffu, tc_wait_err(&empty[s], (f / kKaStages - 1) & 1, abort, &g_kv4_error)))
+          goto landed;
+        const uint32_t have = __ballot_sync(0xffffffffu, page >= 0 && page < a.num_pages);
+        if (lane == 0) {
+          present[s] = have;
+          tc_expect_tx(&full[s], __popc(have) * block);
         }
-      } while (it.next());
-  drained:
+        __syncwarp();
+        if (have >> lane & 1u)
+          ka_copy(ring + s * S::kStage + lane * block, a.pool + ((int64_t)page * a.nkv + head) * block, block, &full[s]);
+      }
+      __syncwarp();
+      if (lane == 0) ka_next(a, cum, &p);
+      __syncwarp();
+    }
+  landed:
     // the copies in flight land before this CTA's shared memory is given away, also when a wait gave up
-    for (uint32_t k = n >= kKaStages ? n - kKaStages : 0; k < n; ++k)
+    for (uint32_t k = f > kKaStages ? f - kKaStages : 0; k < f; ++k)
       tc_wait_err(&full[k % kKaStages], (k / kKaStages) & 1, nullptr, &g_kv4_error);
     return;
   }
@@ -341,26 +351,33 @@ __global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
   const int g = lane >> 2, t = lane & 3;
   bool bad = false;
   uint32_t n = 0;
-  KaWalk it(a, cum);
-  if (it.begin()) do {
-      uint32_t qa[2 * KW][4];
+  KaPos& it = place[0];
+  while (it.live) {
+      if (tid < kKaRows) {
+        const int row = it.tile * kKaRows + tid, i = ka_div_g(a, row);
+        row_token[tid] = row < a.G * a.T ? i : -1;
+        row_head[tid] = it.h * a.G + row - i * a.G;
+      }
+      ka_sync();
       float sc[2];
       int rowpos[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int row = it.tile * kKaRows + g + 8 * k, i = row / a.G;
-        const bool live = row < a.G * a.T;
-        const bf16* p = a.q + ((int64_t)it.b * a.T + (live ? i : 0)) * a.q_stride +
-                        (it.h * a.G + (live ? row % a.G : 0)) * D + t * (D / 4);
+        const int i = row_token[g + 8 * k];
+        const bf16* p = a.q + ((int64_t)it.b * a.T + i) * a.q_stride + row_head[g + 8 * k] * D + t * (D / 4);
         uint32_t h[D / 8];
-        sc[k] = fmaxf(a.scale_log2 * ka_load_q<D / 4>(p, live, h, a.negate), 1e-37f);  // never 0: 0 x -inf
+        sc[k] = fmaxf(a.scale_log2 * ka_load_q<D / 4>(p, i >= 0, h, a.negate), 1e-37f);  // never 0: 0 x -inf
+        // (every warp needs every row's scale; each writes a quarter of the operands)
+        uint32_t* q32 = reinterpret_cast<uint32_t*>(qfrag);
 #pragma unroll
-        for (int s = 0; s < 2 * KW; ++s) {
-          qa[s][k] = h[2 * s];
-          qa[s][2 + k] = h[2 * s + 1];
-        }
-        rowpos[k] = it.x.pos + min(i, a.T - 1);
+        for (int s = 0; s < 2 * KW; ++s)
+          if (s % kKaWarps == warp) {
+            q32[(s * 32 + lane) * 4 + k] = h[2 * s];
+            q32[(s * 32 + lane) * 4 + 2 + k] = h[2 * s + 1];
+          }
+        rowpos[k] = it.x.pos + max(i, 0);
       }
+      ka_sync();
       float o[NV][4];
 #pragma unroll
       for (int i = 0; i < NV; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -369,54 +386,73 @@ __global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
       const int all_hi = it.x.pos + it.x.t0;
       const int all_lo = a.window > 0 ? it.x.pos + it.x.t1 - a.window + 1 : 0;
 
-      for (int c = it.c0; c < it.c1; ++c, ++n) {
+      // (copies of the place's members: behind an address, every barrier would reload them)
+      const int sink_chunks = it.x.sink_chunks, lo_chunk = it.x.lo_chunk, c_end = it.c1, window = a.window, sinks = a.sinks;
+      for (int c = it.c0; c < c_end; ++c, ++n) {
         const uint32_t s = n % kKaStages;
         if (!bad) bad = !__all_sync(0xffffffffu, tc_wait_err(&full[s], (n / kKaStages) & 1, abort, &g_kv4_error));
-        const int key0 = it.first_key(c) + warp * kKaKeys;
-        // 16-row pieces of this warp's rows that were copied
-        const uint32_t here = bad ? 0u : (present[s] >> (warp * kKaPieces)) & ((1u << kKaPieces) - 1u);
+        const int key0 = (c < sink_chunks ? c : lo_chunk + c - sink_chunks) * kKaChunk + warp * kKaKeys;
+        // this warp's 16-row pieces: whether their pages are there, and where
+        const unsigned char* piece[kKaPieces];
+        uint32_t here = 0;
+        if (!bad) {
+          const uint32_t have = present[s];
+#pragma unroll
+          for (int u = 0; u < kKaPieces; ++u) {
+            const int r = warp * kKaKeys + u * 16, j = r >> a.pt_log;
+            here |= (have >> j & 1u) << u;
+            piece[u] = ring + s * S::kStage + j * block + (r & (a.pt - 1)) * (D / 2);
+          }
+        }
         if (here) {
-          const unsigned char* st = ring + s * S::kStage;
           const bool masked = here != (1u << kKaPieces) - 1u || key0 + kKaKeys - 1 > all_hi ||
-                              (key0 < all_lo && key0 + kKaKeys > a.sinks);
+                              (key0 < all_lo && key0 + kKaKeys > sinks);
           auto see = [&](int e, int p) {  // cache row key0 + e from position p
             const int key = key0 + e;
-            return key <= p && (a.window == 0 || key > p - a.window || key < a.sinks) && (here >> (e / 16) & 1u);
+            return key <= p && (window == 0 || key > p - window || key < sinks) && (here >> (e / 16) & 1u);
           };
           // ---- S = Q K^T ----
+          const unsigned char* piece_ks[kKaPieces];
+#pragma unroll
+          for (int u = 0; u < kKaPieces; ++u) {
+            const int r = warp * kKaKeys + u * 16;
+            piece_ks[u] = ring + s * S::kStage + (r >> a.pt_log) * block + kv4_off_ks(a.pt, D) + (r & (a.pt - 1)) * (D / 16);
+          }
           float sa[kKaKeys / 8][4];
-          uint32_t kw[kKaKeys / 8][KW], kf[kKaKeys / 8][2];
+          uint32_t kw[kKaKeys / 8][KW], kf[kKaKeys / 8];
 #pragma unroll
           for (int j = 0; j < kKaKeys / 8; ++j) {
-            const int r = warp * kKaKeys + j * 8 + g;
+            const unsigned char* kc = piece[j / 2] + (j % 2 * 8 + g) * (D / 2);
+            const unsigned char* ks = piece_ks[j / 2] + (j % 2 * 8 + g) * (D / 16);
             if constexpr (D == 128) {
-              const uint4 v = *reinterpret_cast<const uint4*>(st + r * (D / 2) + t * 16);
+              const uint4 v = *reinterpret_cast<const uint4*>(kc + t * 16);
               kw[j][0] = v.x;
               kw[j][1] = v.y;
               kw[j][2] = v.z;
               kw[j][3] = v.w;
-              const uint32_t x = e4m3x2_to_h2(*reinterpret_cast<const uint16_t*>(st + kv4_off_ks(kKaChunk, D) + r * 8 + t * 2));
-              kf[j][0] = __byte_perm(x, 0, 0x1010);
-              kf[j][1] = __byte_perm(x, 0, 0x3232);
+              kf[j] = e4m3x2_to_h2(*reinterpret_cast<const uint16_t*>(ks + t * 2));
             } else {
-              const uint2 v = *reinterpret_cast<const uint2*>(st + r * (D / 2) + t * 8);
+              const uint2 v = *reinterpret_cast<const uint2*>(kc + t * 8);
               kw[j][0] = v.x;
               kw[j][1] = v.y;
-              const uint32_t x = st[kv4_off_ks(kKaChunk, D) + r * 4 + t];
-              kf[j][0] = kf[j][1] = e4m3x2_to_h2(x | (x << 8));
+              const uint32_t x = ks[t];
+              kf[j] = e4m3x2_to_h2(x | (x << 8));
             }
             sa[j][0] = sa[j][1] = sa[j][2] = sa[j][3] = 0.f;
           }
 #pragma unroll
-          for (int k = 0; k < KW; ++k)
+          for (int k = 0; k < KW; ++k) {
+            const uint4 q0 = qfrag[2 * k * 32 + lane], q1 = qfrag[(2 * k + 1) * 32 + lane];
+            const uint32_t qa0[4] = {q0.x, q0.y, q0.z, q0.w}, qa1[4] = {q1.x, q1.y, q1.z, q1.w};
 #pragma unroll
             for (int j = 0; j < kKaKeys / 8; ++j) {
               uint32_t h[4];
               e2m1x8_to_h2(kw[j][k], h);
-              const uint32_t f = kf[j][k * 2 / KW];
-              ka_mma(sa[j], qa[2 * k], hmul2_u(h[0], f), hmul2_u(h[1], f));
-              ka_mma(sa[j], qa[2 * k + 1], hmul2_u(h[2], f), hmul2_u(h[3], f));
+              const uint32_t f = D == 128 ? __byte_perm(kf[j], 0, k < KW / 2 ? 0x1010 : 0x3232) : kf[j];
+              ka_mma(sa[j], qa0, hmul2_u(h[0], f), hmul2_u(h[1], f));
+              ka_mma(sa[j], qa1, hmul2_u(h[2], f), hmul2_u(h[3], f));
             }
+          }
           if (masked) {
 #pragma unroll
             for (int j = 0; j < kKaKeys / 8; ++j)
@@ -461,15 +497,15 @@ __global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
             pa[j / 2][j % 2 * 2 + 1] = ka_h2(p[2], p[3]);
           }
           // ---- O += P V, and the weights' sum as one more column of ones ----
-          const unsigned char* vs = st + kv4_off_vs(kKaChunk, D) + warp * kKaKeys * (D / 16);
-          const unsigned char* vc = st + kv4_off_v(kKaChunk, D) + warp * kKaKeys * (D / 2);
 #pragma unroll
           for (int u = 0; u < kKaPieces; ++u) {
             // this lane's rows 2t, 2t + 1 of both 8-row halves, column g
+            const unsigned char* vc = piece[u] + kv4_off_v(a.pt, D);
+            const unsigned char* vs = piece_ks[u] + a.pt * (D / 16);
             uint32_t sv[4], w[4][VW];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const int r = u * 16 + (k >> 1) * 8 + 2 * t + (k & 1);
+              const int r = (k >> 1) * 8 + 2 * t + (k & 1);
               sv[k] = vs[r * (D / 16) + g * NV / 16];
               if constexpr (D == 128) {
                 const uint2 v = *reinterpret_cast<const uint2*>(vc + r * (D / 2) + g * (NV / 2));
@@ -489,12 +525,12 @@ __global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
                 if (ka_nan_scale(sv[k])) sv[k] = 0;
               }
               if (__any_sync(0xffffffffu, odd)) {
-                for (int e = u * 16; e < u * 16 + 16; ++e)
+                for (int e = 0; e < 16; ++e)
 #pragma unroll
                   for (int k = 0; k < 2; ++k)
 #pragma unroll
                     for (int col = 0; col < 2; ++col)
-                      if (see(e, rowpos[k]) && ka_nan_scale(vs[e * (D / 16) + (2 * t + col) * NV / 16]))
+                      if (see(u * 16 + e, rowpos[k]) && ka_nan_scale(vs[e * (D / 16) + (2 * t + col) * NV / 16]))
 #pragma unroll
                         for (int i = 0; i < NV; ++i) o[i][2 * k + col] = NAN;
               }
@@ -519,137 +555,169 @@ __global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
         if (lane == 0) tc_arrive(&empty[s]);
       }
 
-      // ---- join the four warps ----
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int r = g + 8 * k;
-        if (t == 0) {
-          join_m[warp * kKaRows + r] = m[k];
-          join_l[warp * kKaRows + r] = l[2 * k];
-        }
-        float* row = join + (warp * kKaRows + r) * S::kPad;
-#pragma unroll
-        for (int col = 0; col < 2; ++col)
-#pragma unroll
-          for (int q0 = 0; q0 < NV / 4; ++q0) {
-            const int d = (2 * t + col) * NV + 4 * q0;
-            *reinterpret_cast<float4*>(row + d) =
-                make_float4(o[4 * q0][2 * k + col], o[4 * q0 + 1][2 * k + col], o[4 * q0 + 2][2 * k + col], o[4 * q0 + 3][2 * k + col]);
-          }
-      }
-      ka_sync();
-      // parts of this item: CTAs first .. last of the grid
-      const bool whole = it.c1 - it.c0 == it.x.n;
-      long long u0 = 0, first = 0, parts = 1;
-      if (!whole) {
-        u0 = it.w - it.c0;
-        first = ((u0 + 1) * it.ctas - 1) / it.total;
-        parts = ((u0 + it.x.n) * it.ctas - 1) / it.total - first + 1;
-      }
-      auto slot_of = [&](long long p) {
-        const long long cta = first + p;
-        return 2 * cta + (it.total * cta / it.ctas < u0 ? 1 : 0);
+      // ---- join the four warps: 2 and 3 into 0 and 1, place by place, then those two ----
+      // a column's 16-byte pieces are dealt such that a quarter-warp's accesses meet all banks
+      auto at = [&](int half, int r, int column, int piece) {
+        return reinterpret_cast<float4*>(join + (half * kKaRows + r) * D + (column ^ (r & 1)) * NV +
+                                         4 * (piece ^ (D == 128 ? column >> 1 : column >> 2)));
       };
-      const long long my_part = blockIdx.x - first;
-      float* rec = whole ? nullptr : a.parts + slot_of(my_part) * S::kRecord;
+      ka_sync();  // q's operands are no longer read
+#pragma unroll 1
+      for (int step = 0; step < 2; ++step) {
+        if (warp >> 1 != step) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int r = g + 8 * k;
+            float *jm = join_m + (warp & 1) * kKaRows + r, *jl = join_l + (warp & 1) * kKaRows + r;
+            float mf = 1.f, of = 0.f;
+            if (step) {
+              const float other = *jm, to = fmaxf(m[k], other);
+              mf = m[k] == -INFINITY ? 0.f : ka_exp2(m[k] - to);
+              of = other == -INFINITY ? 0.f : ka_exp2(other - to);
+              m[k] = to;
+              l[2 * k] = l[2 * k] * mf + *jl * of;
+              __syncwarp();
+            }
+            if (t == 0) {
+              *jm = m[k];
+              *jl = l[2 * k];
+            }
+#pragma unroll
+            for (int col = 0; col < 2; ++col)
+#pragma unroll
+              for (int q0 = 0; q0 < NV / 4; ++q0) {
+                float4* e = at(warp & 1, r, 2 * t + col, q0);
+                float4 v = make_float4(o[4 * q0][2 * k + col], o[4 * q0 + 1][2 * k + col], o[4 * q0 + 2][2 * k + col],
+                                       o[4 * q0 + 3][2 * k + col]);
+                if (step) {
+                  const float4 w = *e;
+                  v = make_float4(v.x * mf + w.x * of, v.y * mf + w.y * of, v.z * mf + w.z * of, v.w * mf + w.w * of);
+                }
+                *e = v;
+              }
+          }
+        }
+        ka_sync();
+      }
+      // parts of this item: CTAs first .. first + parts - 1
+      const bool whole = it.c1 - it.c0 == it.x.n;
+      const int u0 = it.w - it.c0, used = it.x.used;
+      int first = 0, parts = 1;
+      if (!whole) {
+        first = ka_owner(it, u0);
+        parts = ka_owner(it, u0 + it.x.n - 1) - first + 1;
+      }
+      // a CTA's range holds one item's end and another's beginning at most: two records per CTA
+      auto slot_of = [&](int p) { return 2 * (first + p) + (ka_range(it, first + p) < u0 ? 1 : 0); };
+      auto out_at = [&](int r, int d) {
+        return a.out + ((int64_t)it.b * a.T + row_token[r]) * a.out_stride + row_head[r] * D + d;
+      };
+      const int my_part = blockIdx.x - first;
+      float* rec = whole ? nullptr : a.parts + (size_t)slot_of(my_part) * S::kRecord;
+#pragma unroll 1
       for (int e = tid; e < kKaRows * D / 4; e += kKaWarps * 32) {
         const int r = e / (D / 4), d = e % (D / 4) * 4;
-        float top = -INFINITY, sum = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kKaWarps; ++w) top = fmaxf(top, join_m[w * kKaRows + r]);
-#pragma unroll
-        for (int w = 0; w < kKaWarps; ++w) {
-          const float mw = join_m[w * kKaRows + r];
-          const float f = mw == -INFINITY ? 0.f : ka_exp2(mw - top);
-          const float4 v = *reinterpret_cast<const float4*>(join + (w * kKaRows + r) * S::kPad + d);
-          sum += join_l[w * kKaRows + r] * f;
-          acc.x += v.x * f;
-          acc.y += v.y * f;
-          acc.z += v.z * f;
-          acc.w += v.w * f;
-        }
+        const float m0 = join_m[r], m1 = join_m[kKaRows + r], top = fmaxf(m0, m1);
+        const float f0 = m0 == -INFINITY ? 0.f : ka_exp2(m0 - top), f1 = m1 == -INFINITY ? 0.f : ka_exp2(m1 - top);
+        const float4 x = *at(0, r, d / NV, d % NV / 4), y = *at(1, r, d / NV, d % NV / 4);
+        const float sum = join_l[r] * f0 + join_l[kKaRows + r] * f1;
+        const float4 v = make_float4(x.x * f0 + y.x * f1, x.y * f0 + y.y * f1, x.z * f0 + y.z * f1, x.w * f0 + y.w * f1);
         if (whole) {
-          ka_store(a, it, D, r, d, acc, sum);
+          const bool on = row_token[r] < used;
+          if (row_token[r] >= 0) ka_store(out_at(r, d), on ? v : make_float4(0.f, 0.f, 0.f, 0.f), on ? sum : 0.f);
         } else {
-          *reinterpret_cast<float4*>(rec + r * D + d) = acc;
+          *reinterpret_cast<float4*>(rec + r * D + d) = v;
           if (d == 0) {
             rec[kKaRows * D + r] = top;
             rec[kKaRows * D + kKaRows + r] = sum;
           }
         }
       }
-      ka_sync();
       // ---- join the CTAs ----
-      long long idx = my_part, count = parts, span = 1;
+      int idx = my_part, count = parts, span = 1;
+#pragma unroll 1
       for (int level = 0; count > 1; ++level) {
-        const long long lead = idx / kKaFan * kKaFan;
-        const int members = (int)min((long long)kKaFan, count - lead);
+        const int lead = idx / kKaFan * kKaFan;
+        const int members = min(kKaFan, count - lead);
         const bool final = count <= kKaFan;
         if (members > 1) {
           __threadfence();
           ka_sync();
           if (tid == 0) {
-            uint32_t* ctr = a.arrived + (long long)level * 2 * gridDim.x + slot_of(lead * span);
+            uint32_t* ctr = a.arrived + level * 2 * gridDim.x + slot_of(lead * span);
             const bool last = atomicAdd(ctr, 1u) == (uint32_t)members - 1;
             if (last) *ctr = 0;
             flags[1] = last;
           }
+          if (tid >= 32 && tid < 32 + kKaFan)  // (the last record again where there are fewer)
+            recs[tid - 32] = a.parts + (size_t)slot_of((lead + min(tid - 32, members - 1)) * span) * S::kRecord;
           ka_sync();
           if (!flags[1]) break;
           __threadfence();
-          float* wgt = join;                                              // [members][16]
-          float** recs = reinterpret_cast<float**>(join + kKaFan * kKaRows);  // [members]
-          if (tid < members) recs[tid] = a.parts + slot_of((lead + tid) * span) * S::kRecord;
-          ka_sync();
-          for (int e = tid; e < members * kKaRows; e += kKaWarps * 32)
-            wgt[e] = __ldcg(recs[e / kKaRows] + kKaRows * D + e % kKaRows);
-          float lp[kKaFan * kKaRows / (kKaWarps * 32)];
+          // thread (part group, row): maxima and sums of two parts
+          float* wgt = join;                    // [16 parts][16 rows]
+          float* sums = join + kKaFan * kKaRows;
+          const int r0 = tid % kKaRows, p0 = tid / kKaRows;  // parts p0 and p0 + 8
+          float mp[2], lp[2];
 #pragma unroll
-          for (int k = 0; k < kKaFan * kKaRows / (kKaWarps * 32); ++k) {
-            const int e = tid + k * kKaWarps * 32;
-            lp[k] = e < members * kKaRows ? __ldcg(recs[e / kKaRows] + kKaRows * D + kKaRows + e % kKaRows) : 0.f;
+          for (int k = 0; k < 2; ++k) {
+            mp[k] = __ldcg(recs[p0 + 8 * k] + kKaRows * D + r0);
+            lp[k] = __ldcg(recs[p0 + 8 * k] + kKaRows * D + kKaRows + r0);
+            if (p0 + 8 * k >= members) mp[k] = -INFINITY;
+            wgt[(p0 + 8 * k) * kKaRows + r0] = mp[k];
           }
           ka_sync();
-          float top = -INFINITY;  // of row tid % 16
-          for (int p = 0; p < members; ++p) top = fmaxf(top, wgt[p * kKaRows + tid % kKaRows]);
-          ka_sync();
-          float* sums = join + kKaFan * kKaRows * 2;  // [members][16]
+          float top = -INFINITY;
 #pragma unroll
-          for (int k = 0; k < kKaFan * kKaRows / (kKaWarps * 32); ++k) {
-            const int e = tid + k * kKaWarps * 32;
-            if (e < members * kKaRows) {
-              const float f = wgt[e] == -INFINITY ? 0.f : ka_exp2(wgt[e] - top);
-              wgt[e] = f;
-              sums[e] = lp[k] * f;
-            }
+          for (int p = 0; p < kKaFan; ++p) top = fmaxf(top, wgt[p * kKaRows + r0]);
+          ka_sync();
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float f = mp[k] == -INFINITY ? 0.f : ka_exp2(mp[k] - top);
+            wgt[(p0 + 8 * k) * kKaRows + r0] = f;
+            sums[(p0 + 8 * k) * kKaRows + r0] = p0 + 8 * k < members ? lp[k] * f : 0.f;
           }
           ka_sync();
           if (tid < kKaRows) {
             float sum = 0.f;
-            for (int p = 0; p < members; ++p) sum += sums[p * kKaRows + tid];
+#pragma unroll
+            for (int p = 0; p < kKaFan; ++p) sum += sums[p * kKaRows + tid];
             join_m[tid] = top;
             join_l[tid] = sum;
           }
           ka_sync();
           float* dst = recs[0];
-          for (int e = tid; e < kKaRows * D / 4; e += kKaWarps * 32) {
-            const int r = e / (D / 4), d = e % (D / 4) * 4;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          // this thread's 16-byte pieces, four parts of each at a time: 16 loads in flight
+          constexpr int kMine = kKaRows * D / 4 / (kKaWarps * 32);
+          float4 acc[kMine];
 #pragma unroll
-            for (int p = 0; p < kKaFan; ++p) {
-              if (p >= members) break;
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(recs[p] + r * D + d));
-              const float f = wgt[p * kKaRows + r];
-              acc.x += v.x * f;
-              acc.y += v.y * f;
-              acc.z += v.z * f;
-              acc.w += v.w * f;
-            }
+          for (int k = 0; k < kMine; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+          for (int q0 = 0; q0 < members; q0 += 4) {
+            float4 v[kMine][4];
+#pragma unroll
+            for (int k = 0; k < kMine; ++k)
+#pragma unroll
+              for (int p = 0; p < 4; ++p)
+                v[k][p] = __ldcg(reinterpret_cast<const float4*>(recs[q0 + p]) + tid + k * kKaWarps * 32);
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+              if (q0 + p < members)
+#pragma unroll
+                for (int k = 0; k < kMine; ++k) {
+                  const float f = wgt[(q0 + p) * kKaRows + (tid + k * kKaWarps * 32) / (D / 4)];
+                  acc[k] = make_float4(acc[k].x + v[k][p].x * f, acc[k].y + v[k][p].y * f, acc[k].z + v[k][p].z * f,
+                                       acc[k].w + v[k][p].w * f);
+                }
+          }
+#pragma unroll
+          for (int k = 0; k < kMine; ++k) {
+            const int e = tid + k * kKaWarps * 32, r = e / (D / 4), d = e % (D / 4) * 4;
             if (final) {
-              ka_store(a, it, D, r, d, acc, join_l[r]);
+              const bool on = row_token[r] < used;
+              if (row_token[r] >= 0) ka_store(out_at(r, d), on ? acc[k] : make_float4(0.f, 0.f, 0.f, 0.f), on ? join_l[r] : 0.f);
             } else {
-              *reinterpret_cast<float4*>(dst + r * D + d) = acc;
+              *reinterpret_cast<float4*>(dst + r * D + d) = acc[k];
               if (d == 0) {
                 dst[kKaRows * D + r] = join_m[r];
                 dst[kKaRows * D + kKaRows + r] = join_l[r];
@@ -662,23 +730,30 @@ __global__ void __launch_bounds__(kKaThreads, 2) k_kv4_attn(KaArgs a) {
         count = (count + kKaFan - 1) / kKaFan;
         span *= kKaFan;
       }
-    } while (it.next());
+      if (a.listed && it.w + it.c1 - it.c0 >= it.w1) break;  // the CTA's last
+      ka_sync();
+      if (tid == 0) ka_next(a, cum, &it);
+      ka_sync();
+  }
 
   // rows of items without a chunk
   if (a.listed) {
-    const long long items = (long long)a.B * a.nkv * a.tiles;
-    for (long long k = blockIdx.x; k < items; k += gridDim.x) {
-      it.item = k;
-      it.locate();
-      if (it.x.n) continue;
-      for (int e = tid; e < kKaRows * D / 4; e += kKaWarps * 32)
-        ka_store(a, it, D, e / (D / 4), e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
+    const int items = a.B * a.nkv * a.tiles;
+    for (int k = blockIdx.x; k < items; k += gridDim.x) {
+      const int tile = k % a.tiles, h = k / a.tiles % a.nkv, b = k / a.tiles / a.nkv;
+      if (ka_tile(a, b, tile).n) continue;
+      for (int e = tid; e < kKaRows * D / 4; e += kKaWarps * 32) {
+        const int row = tile * kKaRows + e / (D / 4), i = row / a.G;
+        if (row < a.G * a.T)
+          *reinterpret_cast<uint2*>(a.out + ((int64_t)b * a.T + i) * a.out_stride + (h * a.G + row - i * a.G) * D +
+                                    e % (D / 4) * 4) = make_uint2(0u, 0u);
+      }
     }
   }
 }
 
-// CTAs of a launch: two per SM, or as many as there are chunks (items) at most.
-static int ka_grid_max() { return 2 * sm_count(); }
+// CTAs of a launch: kKaPerSm per SM, or as many as there are chunks (items) at most.
+static int ka_grid_max() { return kKaPerSm * sm_count(); }
 static size_t ka_arrived_bytes() { return ((size_t)kKaLevels * 2 * ka_grid_max() * 4 + 255) / 256 * 256; }
 static size_t ka_record_bytes(int D) { return (size_t)(kKaRows * D + 2 * kKaRows) * 4; }
 
@@ -688,10 +763,10 @@ static int ka_launch(const KaArgs& a, int grid, cudaStream_t s) {
   int dev = 0;
   JSX_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 128 || !done[dev]) {
-    JSX_CUDA(cudaFuncSetAttribute(k_kv4_attn<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)KaShape<D>::kSmem));
+    JSX_CUDA(cudaFuncSetAttribute(k_kv4_attn<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)KaShape<D>::kStage * kKaStages));
     if (dev >= 0 && dev < 128) done[dev] = true;
   }
-  JSX_CUDA(launch_kernel(k_kv4_attn<D>, dim3(grid), dim3(kKaThreads), KaShape<D>::kSmem, s, a));
+  JSX_CUDA(launch_kernel(k_kv4_attn<D>, dim3(grid), dim3(kKaThreads), KaShape<D>::kStage * kKaStages, s, a));
   return JSX_OK;
 }
 
@@ -714,7 +789,7 @@ extern "C" int jsx_kv4_attn(const void* q, int64_t q_stride, const void* pool, i
   JSX_REQUIRE(q && out && positions, "null pointer argument");
   JSX_KV4_REQUIRE(pool, num_pages, table, table_slots, nkv, head_dim, page_tokens);
   JSX_REQUIRE(nq >= 1 && nq % nkv == 0, "nq=%d is not a multiple of nkv=%d", nq, nkv);
-  JSX_REQUIRE(B >= 1 && T >= 1 && (int64_t)B * T * nq <= INT32_MAX, "B=%d T=%d", B, T);
+  JSX_REQUIRE(B >= 1 && T >= 1 && (int64_t)B * T * nq <= (1 << 30), "B=%d T=%d", B, T);
   JSX_REQUIRE((int64_t)table_slots * page_tokens <= (1 << 30), "a table of %d pages of %d tokens", table_slots, page_tokens);
   JSX_REQUIRE(aligned16(q) && aligned16(out) && q_stride % 8 == 0 && out_stride % 8 == 0 &&
                   q_stride >= (int64_t)nq * head_dim && out_stride >= (int64_t)nq * head_dim,
@@ -743,15 +818,19 @@ extern "C" int jsx_kv4_attn(const void* q, int64_t q_stride, const void* pool, i
   a.T = T;
   a.nkv = nkv;
   a.G = nq / nkv;
+  JSX_REQUIRE((int64_t)a.G * (a.G * T + kKaRows) < (1ll << 32), "%d tokens of %d heads per kv head", T, a.G);
+  a.per_g = (uint32_t)(((1ull << 32) + a.G - 1) / a.G);
   a.tiles = (a.G * T + kKaRows - 1) / kKaRows;
   a.pt = page_tokens;
+  a.pt_log = page_tokens == 16 ? 4 : page_tokens == 32 ? 5 : page_tokens == 64 ? 6 : 7;
   a.window = window < (1 << 30) ? window : 1 << 30;  // (positions are below 2^30)
   a.sinks = sinks;
   a.negate = scale < 0.f ? 0x80000000u : 0u;
   a.scale_log2 = fabsf(scale) * 1.4426950408889634f;
-  a.listed = (int64_t)B * a.tiles <= kKaListMax;
   const int64_t items = (int64_t)B * nkv * a.tiles;
-  const int64_t units = a.listed ? items * (((int64_t)table_slots * page_tokens + kKaChunk - 1) / kKaChunk) : items;
+  const int64_t chunks = items * (((int64_t)table_slots * page_tokens + kKaChunk - 1) / kKaChunk);
+  a.listed = (int64_t)B * a.tiles <= kKaListMax && chunks < (1 << 30);
+  const int64_t units = a.listed ? chunks : items;
   const int grid = (int)(units < ka_grid_max() ? units : ka_grid_max());
   return head_dim == 128 ? ka_launch<128>(a, grid, (cudaStream_t)stream) : ka_launch<64>(a, grid, (cudaStream_t)stream);
 }

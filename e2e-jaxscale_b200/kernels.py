@@ -23,7 +23,9 @@ def _p(t):
 
 
 def _stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    """Handle of torch's current stream on the current device (without building a Stream object,
+    which takes as long as a launch)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _need(t, name, dtype=BF16):
