@@ -234,6 +234,40 @@ __device__ __forceinline__ uint32_t ka_h2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 __device__ __forceinline__ void ka_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }  // the computing warps
+// Shared-memory loads by 32-bit address.  Volatile: the copies that fill the stages are
+// ordered by the barriers alone.
+__device__ __forceinline__ uint4 ka_lds128(uint32_t p) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ka_lds64(uint32_t p) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ka_lds32(uint32_t p) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ka_lds16(uint32_t p) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ka_lds8(uint32_t p) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(p));
+  return v;
+}
+// Bounded wait of a warp, false when it gave up; the waiting loop is out of line.
+__device__ __noinline__ bool ka_wait_slow(uint64_t* b, uint32_t parity, volatile uint32_t* abort) {
+  return __all_sync(0xffffffffu, tc_wait_err(b, parity, abort, &g_kv4_error));
+}
+__device__ __forceinline__ bool ka_wait(uint64_t* b, uint32_t parity, volatile uint32_t* abort) {
+  return __all_sync(0xffffffffu, tc_try_wait<false>(b, parity)) || ka_wait_slow(b, parity, abort);
+}
 __device__ __forceinline__ bool ka_nan_scale(uint32_t s) { return (s & 0x7fu) == 0x7fu; }
 
 // One row's D / 4 values of q at `p` as f16 pairs, scaled by the power of two that brings
@@ -325,7 +359,7 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
         const uint32_t s = f % kKaStages;
         const int page = soon;
         if (c + 1 < c1) soon = look_up(c + 1);
-        if (f >= kKaStages && !__all_sync(0xffffffffu, tc_wait_err(&empty[s], (f / kKaStages - 1) & 1, abort, &g_kv4_error)))
+        if (f >= kKaStages && !ka_wait(&empty[s], (f / kKaStages - 1) & 1, abort))
           goto landed;
         const uint32_t have = __ballot_sync(0xffffffffu, page >= 0 && page < a.num_pages);
         if (lane == 0) {
@@ -349,8 +383,21 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
 
   // ---- the computing warps ----
   const int g = lane >> 2, t = lane & 3;
+  // K's rows are dealt to a tile's columns (column 2i: row i, column 2i + 1: row 4 + (i ^ 1) of
+  // eight) such that neither K's 16-byte nor V's 8-byte loads of a lane group share banks more than twice
+  const int v_row1 = 4 + (t ^ 1), k_row = g & 1 ? 4 + ((g >> 1) ^ 1) : g >> 1;
+  const uint32_t ring_at = s_u32(ring), q_at = s_u32(qfrag) + lane * 16;
+  const uint32_t v_codes = kv4_off_v(a.pt, D), v_scales = a.pt * (D / 16);
+  int piece_page[kKaPieces], piece_code[kKaPieces], piece_scale[kKaPieces];
+#pragma unroll
+  for (int u = 0; u < kKaPieces; ++u) {
+    const int r = warp * kKaKeys + u * 16;
+    piece_page[u] = r >> a.pt_log;
+    piece_code[u] = piece_page[u] * block + (r & (a.pt - 1)) * (D / 2);
+    piece_scale[u] = piece_page[u] * block + kv4_off_ks(a.pt, D) + (r & (a.pt - 1)) * (D / 16);
+  }
   bool bad = false;
-  uint32_t n = 0;
+  uint32_t stage = 0, phase = 0;
   KaPos& it = place[0];
   while (it.live) {
       if (tid < kKaRows) {
@@ -386,23 +433,19 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
       const int all_hi = it.x.pos + it.x.t0;
       const int all_lo = a.window > 0 ? it.x.pos + it.x.t1 - a.window + 1 : 0;
 
-      // (copies of the place's members: behind an address, every barrier would reload them)
       const int sink_chunks = it.x.sink_chunks, lo_chunk = it.x.lo_chunk, c_end = it.c1, window = a.window, sinks = a.sinks;
-      for (int c = it.c0; c < c_end; ++c, ++n) {
-        const uint32_t s = n % kKaStages;
-        if (!bad) bad = !__all_sync(0xffffffffu, tc_wait_err(&full[s], (n / kKaStages) & 1, abort, &g_kv4_error));
+      for (int c = it.c0; c < c_end; ++c) {
+        if (!bad) bad = !ka_wait(&full[stage], phase, abort);
         const int key0 = (c < sink_chunks ? c : lo_chunk + c - sink_chunks) * kKaChunk + warp * kKaKeys;
         // this warp's 16-row pieces: whether their pages are there, and where
-        const unsigned char* piece[kKaPieces];
-        uint32_t here = 0;
-        if (!bad) {
-          const uint32_t have = present[s];
+        const uint32_t st = ring_at + stage * S::kStage;
+        const uint32_t have = bad ? 0u : present[stage];
+        uint32_t here = 0, piece[kKaPieces], piece_ks[kKaPieces];
 #pragma unroll
-          for (int u = 0; u < kKaPieces; ++u) {
-            const int r = warp * kKaKeys + u * 16, j = r >> a.pt_log;
-            here |= (have >> j & 1u) << u;
-            piece[u] = ring + s * S::kStage + j * block + (r & (a.pt - 1)) * (D / 2);
-          }
+        for (int u = 0; u < kKaPieces; ++u) {
+          here |= (have >> piece_page[u] & 1u) << u;
+          piece[u] = st + piece_code[u];
+          piece_ks[u] = st + piece_scale[u];
         }
         if (here) {
           const bool masked = here != (1u << kKaPieces) - 1u || key0 + kKaKeys - 1 > all_hi ||
@@ -412,37 +455,31 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
             return key <= p && (window == 0 || key > p - window || key < sinks) && (here >> (e / 16) & 1u);
           };
           // ---- S = Q K^T ----
-          const unsigned char* piece_ks[kKaPieces];
-#pragma unroll
-          for (int u = 0; u < kKaPieces; ++u) {
-            const int r = warp * kKaKeys + u * 16;
-            piece_ks[u] = ring + s * S::kStage + (r >> a.pt_log) * block + kv4_off_ks(a.pt, D) + (r & (a.pt - 1)) * (D / 16);
-          }
           float sa[kKaKeys / 8][4];
           uint32_t kw[kKaKeys / 8][KW], kf[kKaKeys / 8];
 #pragma unroll
           for (int j = 0; j < kKaKeys / 8; ++j) {
-            const unsigned char* kc = piece[j / 2] + (j % 2 * 8 + g) * (D / 2);
-            const unsigned char* ks = piece_ks[j / 2] + (j % 2 * 8 + g) * (D / 16);
+            const uint32_t kc = piece[j / 2] + (j % 2 * 8) * (D / 2) + k_row * (D / 2) + t * (D / 8);
+            const uint32_t ks = piece_ks[j / 2] + (j % 2 * 8) * (D / 16) + k_row * (D / 16) + t * (D / 64);
             if constexpr (D == 128) {
-              const uint4 v = *reinterpret_cast<const uint4*>(kc + t * 16);
+              const uint4 v = ka_lds128(kc);
               kw[j][0] = v.x;
               kw[j][1] = v.y;
               kw[j][2] = v.z;
               kw[j][3] = v.w;
-              kf[j] = e4m3x2_to_h2(*reinterpret_cast<const uint16_t*>(ks + t * 2));
+              kf[j] = e4m3x2_to_h2(ka_lds16(ks));
             } else {
-              const uint2 v = *reinterpret_cast<const uint2*>(kc + t * 8);
+              const uint2 v = ka_lds64(kc);
               kw[j][0] = v.x;
               kw[j][1] = v.y;
-              const uint32_t x = ks[t];
+              const uint32_t x = ka_lds8(ks);
               kf[j] = e4m3x2_to_h2(x | (x << 8));
             }
             sa[j][0] = sa[j][1] = sa[j][2] = sa[j][3] = 0.f;
           }
 #pragma unroll
           for (int k = 0; k < KW; ++k) {
-            const uint4 q0 = qfrag[2 * k * 32 + lane], q1 = qfrag[(2 * k + 1) * 32 + lane];
+            const uint4 q0 = ka_lds128(q_at + 2 * k * 512), q1 = ka_lds128(q_at + (2 * k + 1) * 512);
             const uint32_t qa0[4] = {q0.x, q0.y, q0.z, q0.w}, qa1[4] = {q1.x, q1.y, q1.z, q1.w};
 #pragma unroll
             for (int j = 0; j < kKaKeys / 8; ++j) {
@@ -458,7 +495,7 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
             for (int j = 0; j < kKaKeys / 8; ++j)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (!see(j * 8 + 2 * t + (e & 1), rowpos[e >> 1])) sa[j][e] = -INFINITY;
+                if (!see(j * 8 + (e & 1 ? v_row1 : t), rowpos[e >> 1])) sa[j][e] = -INFINITY;
           }
           // ---- running reference, weights ----
           bool move = false;
@@ -500,19 +537,19 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
 #pragma unroll
           for (int u = 0; u < kKaPieces; ++u) {
             // this lane's rows 2t, 2t + 1 of both 8-row halves, column g
-            const unsigned char* vc = piece[u] + kv4_off_v(a.pt, D);
-            const unsigned char* vs = piece_ks[u] + a.pt * (D / 16);
+            const uint32_t vc = piece[u] + v_codes, vs = piece_ks[u] + v_scales;
+            // this lane's two rows of both 8-row halves, column g
             uint32_t sv[4], w[4][VW];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const int r = (k >> 1) * 8 + 2 * t + (k & 1);
-              sv[k] = vs[r * (D / 16) + g * NV / 16];
+              const int r = (k >> 1) * 8 + (k & 1 ? v_row1 : t);
+              sv[k] = ka_lds8(vs + r * (D / 16) + g * NV / 16);
               if constexpr (D == 128) {
-                const uint2 v = *reinterpret_cast<const uint2*>(vc + r * (D / 2) + g * (NV / 2));
+                const uint2 v = ka_lds64(vc + r * (D / 2) + g * (NV / 2));
                 w[k][0] = v.x;
                 w[k][1] = v.y;
               } else {
-                w[k][0] = *reinterpret_cast<const uint32_t*>(vc + r * (D / 2) + g * (NV / 2));
+                w[k][0] = ka_lds32(vc + r * (D / 2) + g * (NV / 2));
               }
             }
             if (masked) {
@@ -530,7 +567,7 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
                   for (int k = 0; k < 2; ++k)
 #pragma unroll
                     for (int col = 0; col < 2; ++col)
-                      if (see(u * 16 + e, rowpos[k]) && ka_nan_scale(vs[e * (D / 16) + (2 * t + col) * NV / 16]))
+                      if (see(u * 16 + e, rowpos[k]) && ka_nan_scale(ka_lds8(vs + e * (D / 16) + (2 * t + col) * NV / 16)))
 #pragma unroll
                         for (int i = 0; i < NV; ++i) o[i][2 * k + col] = NAN;
               }
@@ -552,7 +589,11 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
           }
         }
         __syncwarp();
-        if (lane == 0) tc_arrive(&empty[s]);
+        if (lane == 0) tc_arrive(&empty[stage]);
+        if (++stage == kKaStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
       }
 
       // ---- join the four warps: 2 and 3 into 0 and 1, place by place, then those two ----
