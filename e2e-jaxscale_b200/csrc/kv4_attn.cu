@@ -39,8 +39,8 @@ constexpr int kKaWarps = 4;     // computing warps, 32 cache rows of a chunk eac
 constexpr int kKaKeys = kKaChunk / kKaWarps;
 constexpr int kKaPieces = kKaKeys / 16;
 constexpr int kKaThreads = (kKaWarps + 1) * 32;  // and one that copies
-constexpr int kKaPerSm = 3;     // CTAs per SM
-constexpr int kKaStages = 3;
+constexpr int kKaPerSm = 2;     // CTAs per SM (three of 128 registers a thread measured slower: 73 against 70 us)
+constexpr int kKaStages = 4;
 constexpr int kKaFan = 16;      // parts joined at once
 constexpr int kKaLevels = 3;    // 16^3 parts of an item at most
 constexpr int kKaListMax = 512;   // (sequence, row tile) pairs up to which the chunk list is cut into ranges
@@ -310,8 +310,8 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
   constexpr int NV = D / 8;       // n tiles of O = dimensions per column
   constexpr int VW = D / 64;      // words of codes per lane and V row
   extern __shared__ __align__(128) unsigned char ring[];
-  __shared__ __align__(16) float join[2 * kKaRows * D];  // two warps' outputs; before that q as MMA operands [D / 16][32 lanes]
-  __shared__ float join_m[2 * kKaRows], join_l[2 * kKaRows];
+  __shared__ __align__(16) float join[kKaWarps * kKaRows * D];  // the warps' outputs; before that q as MMA operands [D / 16][32 lanes]
+  __shared__ float join_m[kKaWarps * kKaRows], join_l[kKaWarps * kKaRows];
   __shared__ int cum[kKaListMax + 1];
   __shared__ KaPos place[2];
   __shared__ uint64_t full[kKaStages], empty[kKaStages];
@@ -596,50 +596,28 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
         }
       }
 
-      // ---- join the four warps: 2 and 3 into 0 and 1, place by place, then those two ----
+      // ---- join the four warps ----
       // a column's 16-byte pieces are dealt such that a quarter-warp's accesses meet all banks
-      auto at = [&](int half, int r, int column, int piece) {
-        return reinterpret_cast<float4*>(join + (half * kKaRows + r) * D + (column ^ (r & 1)) * NV +
+      auto at = [&](int w, int r, int column, int piece) {
+        return reinterpret_cast<float4*>(join + (w * kKaRows + r) * D + (column ^ (r & 1)) * NV +
                                          4 * (piece ^ (D == 128 ? column >> 1 : column >> 2)));
       };
       ka_sync();  // q's operands are no longer read
-#pragma unroll 1
-      for (int step = 0; step < 2; ++step) {
-        if (warp >> 1 != step) {
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int r = g + 8 * k;
-            float *jm = join_m + (warp & 1) * kKaRows + r, *jl = join_l + (warp & 1) * kKaRows + r;
-            float mf = 1.f, of = 0.f;
-            if (step) {
-              const float other = *jm, to = fmaxf(m[k], other);
-              mf = m[k] == -INFINITY ? 0.f : ka_exp2(m[k] - to);
-              of = other == -INFINITY ? 0.f : ka_exp2(other - to);
-              m[k] = to;
-              l[2 * k] = l[2 * k] * mf + *jl * of;
-              __syncwarp();
-            }
-            if (t == 0) {
-              *jm = m[k];
-              *jl = l[2 * k];
-            }
-#pragma unroll
-            for (int col = 0; col < 2; ++col)
-#pragma unroll
-              for (int q0 = 0; q0 < NV / 4; ++q0) {
-                float4* e = at(warp & 1, r, 2 * t + col, q0);
-                float4 v = make_float4(o[4 * q0][2 * k + col], o[4 * q0 + 1][2 * k + col], o[4 * q0 + 2][2 * k + col],
-                                       o[4 * q0 + 3][2 * k + col]);
-                if (step) {
-                  const float4 w = *e;
-                  v = make_float4(v.x * mf + w.x * of, v.y * mf + w.y * of, v.z * mf + w.z * of, v.w * mf + w.w * of);
-                }
-                *e = v;
-              }
-          }
+      for (int k = 0; k < 2; ++k) {
+        const int r = g + 8 * k;
+        if (t == 0) {
+          join_m[warp * kKaRows + r] = m[k];
+          join_l[warp * kKaRows + r] = l[2 * k];
         }
-        ka_sync();
+#pragma unroll
+        for (int col = 0; col < 2; ++col)
+#pragma unroll
+          for (int q0 = 0; q0 < NV / 4; ++q0)
+            *at(warp, r, 2 * t + col, q0) = make_float4(o[4 * q0][2 * k + col], o[4 * q0 + 1][2 * k + col],
+                                                        o[4 * q0 + 2][2 * k + col], o[4 * q0 + 3][2 * k + col]);
       }
+      ka_sync();
       // parts of this item: CTAs first .. first + parts - 1
       const bool whole = it.c1 - it.c0 == it.x.n;
       const int u0 = it.w - it.c0, used = it.x.used;
@@ -658,11 +636,17 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
 #pragma unroll 1
       for (int e = tid; e < kKaRows * D / 4; e += kKaWarps * 32) {
         const int r = e / (D / 4), d = e % (D / 4) * 4;
-        const float m0 = join_m[r], m1 = join_m[kKaRows + r], top = fmaxf(m0, m1);
-        const float f0 = m0 == -INFINITY ? 0.f : ka_exp2(m0 - top), f1 = m1 == -INFINITY ? 0.f : ka_exp2(m1 - top);
-        const float4 x = *at(0, r, d / NV, d % NV / 4), y = *at(1, r, d / NV, d % NV / 4);
-        const float sum = join_l[r] * f0 + join_l[kKaRows + r] * f1;
-        const float4 v = make_float4(x.x * f0 + y.x * f1, x.y * f0 + y.y * f1, x.z * f0 + y.z * f1, x.w * f0 + y.w * f1);
+        float top = -INFINITY, sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kKaWarps; ++w) top = fmaxf(top, join_m[w * kKaRows + r]);
+#pragma unroll
+        for (int w = 0; w < kKaWarps; ++w) {
+          const float mw = join_m[w * kKaRows + r], f = mw == -INFINITY ? 0.f : ka_exp2(mw - top);
+          const float4 x = *at(w, r, d / NV, d % NV / 4);
+          sum += join_l[w * kKaRows + r] * f;
+          v = make_float4(v.x + x.x * f, v.y + x.y * f, v.z + x.z * f, v.w + x.w * f);
+        }
         if (whole) {
           const bool on = row_token[r] < used;
           if (row_token[r] >= 0) ka_store(out_at(r, d), on ? v : make_float4(0.f, 0.f, 0.f, 0.f), on ? sum : 0.f);
