@@ -12,8 +12,8 @@
 //   compact  live pages move into the free ones below, so that the pool's upper
 //            part becomes free.
 //
-// The bookkeeping of a call is one cluster of 8 CTAs (8192 threads): its phases
-// depend on one another (count, rank, assign) and the cluster's barrier orders
+// The bookkeeping of a call is one CTA, or one cluster of 8 (8192 threads) for large pools:
+// its phases depend on one another (count, rank, assign) and the barrier orders
 // them without further launches.  Ranks are prefix sums over page and sequence
 // order, so the pages chosen do not depend on the order of execution.  Page
 // bytes move in a second launch, one (page, layer) unit per CTA at a time,
@@ -26,8 +26,7 @@ namespace jsx {
 
 constexpr int kPgCtas = 8;
 constexpr int kPgThreads = 1024;
-constexpr int kPgWarps = kPgCtas * kPgThreads / 32;
-constexpr int kPgCopyThreads = 256;
+constexpr int kPgCopyThreads = 288;  // pages are multiples of 72 vectors of 16 bytes; 1152 (2 kv heads, 64 x 128) are four each
 
 // workspace (int32): header [16], cnt [S], base [S], src [cap], dst [cap], ref [cap]
 constexpr int kPgHeader = 16;  // [0] pages in the list
@@ -59,12 +58,19 @@ __device__ __forceinline__ uint32_t pg_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-// barrier over the cluster; global and shared writes before it are visible after it
+// barrier over the kCtas CTAs; global and shared writes before it are visible after it
+template <int kCtas>
 __device__ __forceinline__ void pg_sync() {
+  if constexpr (kCtas == 1) {
+    __syncthreads();
+    return;
+  }
   __threadfence();
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+template <int kCtas>
 __device__ __forceinline__ int pg_peer(const int* p, uint32_t rank) {
+  if constexpr (kCtas == 1) return *p;
   uint32_t a, v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -95,9 +101,10 @@ __device__ __forceinline__ int pg_scan(int v, int* warp_sums, int* total) {
   *total = warp_sums[31];
   return x - v + (warp > 0 ? warp_sums[warp - 1] : 0);
 }
-// this thread's pages [lo, hi) of the cluster's partition of [0, P)
+// this thread's pages [lo, hi) of the CTAs' partition of [0, P)
+template <int kCtas>
 __device__ __forceinline__ void pg_range(int P, uint32_t cta, int* lo, int* hi) {
-  const int per = (P + kPgCtas * kPgThreads - 1) / (kPgCtas * kPgThreads);
+  const int per = (P + kCtas * kPgThreads - 1) / (kCtas * kPgThreads);
   const long long l = (long long)(cta * kPgThreads + threadIdx.x) * per;
   *lo = (int)(l < P ? l : P);
   *hi = (int)(l + per < P ? l + per : P);
@@ -113,20 +120,21 @@ struct PgForkArgs {
   int S, slots, P;
 };
 
-__global__ void __cluster_dims__(kPgCtas, 1, 1) __launch_bounds__(kPgThreads) k_pages_fork(PgForkArgs a) {
+template <int kCtas>
+__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kPgThreads) k_pages_fork(PgForkArgs a) {
   pdl_wait();
   const uint32_t cta = pg_rank();
   const int lane = threadIdx.x & 31, w0 = cta * (kPgThreads / 32) + (threadIdx.x >> 5);
-  for (int p = cta * kPgThreads + threadIdx.x; p < a.P; p += kPgCtas * kPgThreads) a.refs_out[p] = a.refs[p];
-  for (int s = w0; s < a.S; s += kPgWarps) {
+  for (int p = cta * kPgThreads + threadIdx.x; p < a.P; p += kCtas * kPgThreads) a.refs_out[p] = a.refs[p];
+  for (int s = w0; s < a.S; s += kCtas * kPgThreads / 32) {
     const int par = a.parent[s];
     const int h = par >= 0 && par < a.S ? pg_held(a.held, par, a.slots) : 0;
     for (int i = lane; i < a.slots; i += 32)
       a.table_out[(size_t)s * a.slots + i] = i < h ? a.table[(size_t)par * a.slots + i] : -1;
     if (lane == 0) a.held_out[s] = h;
   }
-  pg_sync();  // refs_out holds the old counts
-  for (int s = w0; s < a.S; s += kPgWarps) {
+  pg_sync<kCtas>();  // refs_out holds the old counts
+  for (int s = w0; s < a.S; s += kCtas * kPgThreads / 32) {
     const int par = a.parent[s];
     if (par == s) continue;
     const int h0 = pg_held(a.held, s, a.slots);
@@ -167,7 +175,8 @@ __device__ __forceinline__ PgRow pg_row(const PgResizeArgs& a, int s) {
   return r;
 }
 
-__global__ void __cluster_dims__(kPgCtas, 1, 1) __launch_bounds__(kPgThreads) k_pages_resize(PgResizeArgs a) {
+template <int kCtas>
+__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kPgThreads) k_pages_resize(PgResizeArgs a) {
   __shared__ int warp_sums[32];
   __shared__ int mine;
   pdl_wait();
@@ -176,7 +185,7 @@ __global__ void __cluster_dims__(kPgCtas, 1, 1) __launch_bounds__(kPgThreads) k_
   auto writable = [&](int page) { return page >= 0 && page < a.P && a.refs[page] <= 1; };
 
   // pages that every sequence takes
-  for (int s = w0; s < a.S; s += kPgWarps) {
+  for (int s = w0; s < a.S; s += kCtas * kPgThreads / 32) {
     const PgRow r = pg_row(a, s);
     int n = 0;
     for (int i = r.first + lane; i < min(r.before, r.after); i += 32) n += !writable(a.table[(size_t)s * a.slots + i]);
@@ -189,15 +198,15 @@ __global__ void __cluster_dims__(kPgCtas, 1, 1) __launch_bounds__(kPgThreads) k_
   }
   // free pages of this thread's range
   int lo, hi, total_free;
-  pg_range(a.P, cta, &lo, &hi);
+  pg_range<kCtas>(a.P, cta, &lo, &hi);
   int nfree = 0;
   for (int p = lo; p < hi; ++p) nfree += a.refs[p] == 0;
   int rank = pg_scan(nfree, warp_sums, &total_free);
   if (tid == 0) mine = total_free;
-  pg_sync();
+  pg_sync<kCtas>();
   int found = 0;
-  for (int r = 0; r < kPgCtas; ++r) {
-    const int n = pg_peer(&mine, r);
+  for (int r = 0; r < kCtas; ++r) {
+    const int n = pg_peer<kCtas>(&mine, r);
     if (r < (int)cta) rank += n;
     found += n;
   }
@@ -212,7 +221,7 @@ __global__ void __cluster_dims__(kPgCtas, 1, 1) __launch_bounds__(kPgThreads) k_
   int base = pg_scan(n, warp_sums, &total);
   pg_scan(over, warp_sums, &total_over);
   const int missing = max(total - found, 0) + total_over;
-  pg_sync();  // everyone has read cnt and base
+  pg_sync<kCtas>();  // everyone has read cnt and base
   if (missing == 0) {
     for (int p = lo; p < hi && rank < total; ++p)
       if (a.refs[p] == 0) a.ws.dst[rank++] = p;
@@ -226,12 +235,12 @@ __global__ void __cluster_dims__(kPgCtas, 1, 1) __launch_bounds__(kPgThreads) k_
     a.ws.head[0] = missing ? 0 : total;
     *a.missing = missing;
   }
-  pg_sync();
+  pg_sync<kCtas>();
   if (missing) return;  // all or nothing
 
   // Whether a page is shared is asked of the counts before this call: they are
   // changed only after every warp of the cluster has its answers.
-  for (int s = w0; s < a.S; s += kPgWarps) {
+  for (int s = w0; s < a.S; s += kCtas * kPgThreads / 32) {
     const PgRow r = pg_row(a, s);
     int at = a.ws.base[s];
     for (int i0 = r.first; i0 < r.after; i0 += 32) {
@@ -253,12 +262,12 @@ __global__ void __cluster_dims__(kPgCtas, 1, 1) __launch_bounds__(kPgThreads) k_
       at += __popc(m);
     }
   }
-  pg_sync();
-  for (int k = cta * kPgThreads + tid; k < total; k += kPgCtas * kPgThreads) {
+  pg_sync<kCtas>();
+  for (int k = cta * kPgThreads + tid; k < total; k += kCtas * kPgThreads) {
     a.refs[a.ws.dst[k]] = 1;
     if (a.ws.ref[k] >= 0) atomicSub(&a.refs[a.ws.ref[k]], 1);
   }
-  for (int s = w0; s < a.S; s += kPgWarps) {
+  for (int s = w0; s < a.S; s += kCtas * kPgThreads / 32) {
     const PgRow r = pg_row(a, s);
     for (int i = r.after + lane; i < r.before; i += 32) {
       int32_t* e = &a.table[(size_t)s * a.slots + i];
@@ -278,20 +287,21 @@ struct PgCompactArgs {
 };
 
 // refs_out may be refs: every count is read before the last barrier, written after it.
-__global__ void __cluster_dims__(kPgCtas, 1, 1) __launch_bounds__(kPgThreads) k_pages_plan(PgCompactArgs a) {
+template <int kCtas>
+__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kPgThreads) k_pages_plan(PgCompactArgs a) {
   __shared__ int warp_sums[32];
   __shared__ int mine[3];
   pdl_wait();
   const uint32_t cta = pg_rank();
   const int tid = threadIdx.x;
   int lo, hi, n = 0, total;
-  pg_range(a.P, cta, &lo, &hi);
+  pg_range<kCtas>(a.P, cta, &lo, &hi);
   for (int p = lo; p < hi; ++p) n += a.refs[p] > 0;
   pg_scan(n, warp_sums, &total);
   if (tid == 0) mine[0] = total;
-  pg_sync();
+  pg_sync<kCtas>();
   int live = 0;
-  for (int r = 0; r < kPgCtas; ++r) live += pg_peer(&mine[0], r);
+  for (int r = 0; r < kCtas; ++r) live += pg_peer<kCtas>(&mine[0], r);
   int holes = 0, movers = 0;
   for (int p = lo; p < hi; ++p) {
     const bool on = a.refs[p] > 0;
@@ -302,10 +312,10 @@ __global__ void __cluster_dims__(kPgCtas, 1, 1) __launch_bounds__(kPgThreads) k_
   if (tid == 0) mine[1] = total;
   int mover_rank = pg_scan(movers, warp_sums, &total);
   if (tid == 0) mine[2] = total;
-  pg_sync();
+  pg_sync<kCtas>();
   int moved = 0;
-  for (int r = 0; r < kPgCtas; ++r) {
-    const int h = pg_peer(&mine[1], r), m = pg_peer(&mine[2], r);
+  for (int r = 0; r < kCtas; ++r) {
+    const int h = pg_peer<kCtas>(&mine[1], r), m = pg_peer<kCtas>(&mine[2], r);
     if (r < (int)cta) {
       hole_rank += h;
       mover_rank += m;
@@ -321,7 +331,7 @@ __global__ void __cluster_dims__(kPgCtas, 1, 1) __launch_bounds__(kPgThreads) k_
     }
   }
   if (cta == 0 && tid == 0) a.ws.head[0] = moved;
-  pg_sync();
+  pg_sync<kCtas>();
   for (int p = lo; p < hi; ++p) {
     const int r = a.refs[p];
     if (p >= live) {
@@ -334,8 +344,8 @@ __global__ void __cluster_dims__(kPgCtas, 1, 1) __launch_bounds__(kPgThreads) k_
       a.remap[p] = -1;
     }
   }
-  pg_sync();  // with refs_out == refs, a hole's count is read above and written below
-  for (int k = cta * kPgThreads + tid; k < moved; k += kPgCtas * kPgThreads) {
+  pg_sync<kCtas>();  // with refs_out == refs, a hole's count is read above and written below
+  for (int k = cta * kPgThreads + tid; k < moved; k += kCtas * kPgThreads) {
     a.refs_out[a.ws.dst[k]] = a.ws.ref[k];
     a.remap[a.ws.src[k]] = a.ws.dst[k];
   }
@@ -363,15 +373,34 @@ __global__ void __launch_bounds__(kPgCopyThreads) k_pages_copy(PgCopyArgs a) {
       a.table_out[e] = i < pg_held(a.held, s, a.slots) && p >= 0 && p < a.P ? a.remap[p] : -1;
     }
   }
+  // a CTA takes as many (page, layer) units at once as its threads cover; all of a
+  // thread's loads are in flight before its first store
+  const int together = a.page_vecs < kPgCopyThreads ? kPgCopyThreads / (int)a.page_vecs : 1;
+  const int mine = together > 1 ? tid / (int)a.page_vecs : 0, v0 = tid - mine * (int)a.page_vecs;
   const long long units = (long long)a.ws.head[0] * a.layers;
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
+  if (mine >= together) return;
+  for (long long u = (long long)blockIdx.x * together + mine; u < units; u += (long long)gridDim.x * together) {
     const int k = (int)(u / a.layers), l = (int)(u % a.layers);
     const int from = a.ws.src[k];
     if (from < 0) continue;
     const uint4* s = a.pool + (size_t)l * a.layer_vecs + (size_t)from * a.page_vecs;
     uint4* d = a.pool + (size_t)l * a.layer_vecs + (size_t)a.ws.dst[k] * a.page_vecs;
-    for (size_t v = tid; v < a.page_vecs; v += kPgCopyThreads) d[v] = s[v];
+    for (size_t v = v0; v < a.page_vecs; v += 4 * kPgCopyThreads) {
+      uint4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (v + i * kPgCopyThreads < a.page_vecs) x[i] = ld_stream(s + v + i * kPgCopyThreads);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (v + i * kPgCopyThreads < a.page_vecs) d[v + i * kPgCopyThreads] = x[i];
+    }
   }
+}
+
+// One CTA where it has at most 8 pages and 8 table entries a thread to look at: a CTA's
+// barrier is then cheaper than a cluster's.
+static int pages_ctas(int S, int slots, int P) {
+  return P <= 8 * kPgThreads && (long long)S * slots <= 8 * kPgThreads ? 1 : kPgCtas;
 }
 
 static int pages_check(const void* table, const void* held, const void* refs, int S, int slots, int P) {
@@ -417,7 +446,9 @@ extern "C" int jsx_pages_fork(const int32_t* table, const int32_t* held, const i
   JSX_REQUIRE(parent && table_out && held_out && refs_out, "null pointer argument");
   JSX_REQUIRE(table_out != table && held_out != held, "table_out and held_out must not be table and held");
   PgForkArgs a = {table, held, refs, parent, table_out, held_out, refs_out, sequences, slots, num_pages};
-  JSX_CUDA(launch_kernel(k_pages_fork, dim3(kPgCtas), dim3(kPgThreads), 0, (cudaStream_t)stream, a));
+  const int n = pages_ctas(sequences, slots, num_pages);
+  JSX_CUDA(launch_kernel(n == 1 ? k_pages_fork<1> : k_pages_fork<kPgCtas>, dim3(n), dim3(kPgThreads), 0,
+                         (cudaStream_t)stream, a));
   return JSX_OK;
 }
 
@@ -442,7 +473,9 @@ extern "C" int jsx_pages_resize(int32_t* table, int32_t* held, int32_t* refs, co
   a.slots = slots;
   a.P = num_pages;
   a.pt = page_tokens;
-  JSX_CUDA(launch_kernel(k_pages_resize, dim3(kPgCtas), dim3(kPgThreads), 0, (cudaStream_t)stream, a));
+  const int n = pages_ctas(sequences, slots, num_pages);
+  JSX_CUDA(launch_kernel(n == 1 ? k_pages_resize<1> : k_pages_resize<kPgCtas>, dim3(n), dim3(kPgThreads), 0,
+                         (cudaStream_t)stream, a));
   PgCopyArgs c = {};
   c.ws = a.ws;
   return pages_copy(c, pool, layers, page_bytes, num_pages, (cudaStream_t)stream);
@@ -467,7 +500,9 @@ extern "C" int jsx_pages_compact(const int32_t* table, const int32_t* held, cons
   a.S = sequences;
   a.slots = slots;
   a.P = num_pages;
-  JSX_CUDA(launch_kernel(k_pages_plan, dim3(kPgCtas), dim3(kPgThreads), 0, (cudaStream_t)stream, a));
+  const int n = pages_ctas(sequences, slots, num_pages);
+  JSX_CUDA(launch_kernel(n == 1 ? k_pages_plan<1> : k_pages_plan<kPgCtas>, dim3(n), dim3(kPgThreads), 0,
+                         (cudaStream_t)stream, a));
   PgCopyArgs c = {};
   c.ws = a.ws;
   c.table = table;

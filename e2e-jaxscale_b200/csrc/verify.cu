@@ -16,10 +16,14 @@
 // running sum exceeds floor(u total), u taken to 24 bits.  The floor costs a row
 // at most V 2^-41 of its mass (7e-8 at 151552 tokens).
 //
-// Two launches, each one cluster of 8 CTAs per row (stats: every row; draw: one
-// row per sequence): a row of 151552 bf16 logits is 303 KB, an eighth of it is read
-// from memory once and the second pass (the sum after the maximum) hits L1.
-// Temperature 0 is greedy: p is 1 at the lowest index of the maximum.
+// Three launches over slices of rows: the rows' maxima, their sums, and the weights of the
+// one row per sequence that a token is drawn from, summed per step of 32 vectors; the last
+// CTA of a sequence finds the step with the crossing and weighs it again.  Slices meet in
+// integer atomics (maximum, sum), so they need no order and no wait; the second pass
+// over the logits comes from L2 (at most 126 MB of it).  At temperature 0 (greedy: p is
+// 1 at the lowest index of the maximum) nothing is weighed.
+// Bound: the exponentials' instructions (about 22 per logit with the exact sum) above
+// the bytes from some 20 rows on; launches below.
 // NaN logits and a row's -inf entries have no mass; a row with no mass at all, or
 // with +inf, accepts nothing and draws token -1 (greedy takes +inf as the maximum).
 #include <math.h>
@@ -29,17 +33,20 @@
 
 namespace jsx {
 
-constexpr int kVfCtas = 8;
-constexpr int kVfThreads = 512;
+constexpr int kVfThreads = 256;
+constexpr int kVfWarps = kVfThreads / 32;
 constexpr int kVfMaxDraft = 31;
 constexpr int kVfMaxVocab = 1 << 20;
+constexpr int kVfMaxPer = 8;  // vectors a thread weighs before its warp adds them up (32 bits hold 15 x 8 x 32 x 2^20)
 
-struct VfRow {  // per (sequence, position), written by the first kernel
+// Per (sequence, position).  Zero between calls: the slices add and take maxima.
+struct VfRow {
   unsigned long long sum;  // Z; 0: no distribution
-  float max;
-  int best;  // temperature 0: argmax, -1 none
-  int ok;    // draft accepted (positions < n_draft)
-  int pad;
+  uint32_t top;            // order key of the largest logit, 0: none
+  uint32_t best;           // temperature 0: ~index of the first maximum, 0: none
+  float logit, q;          // of the drafted token
+  int drafted;             // there is one, inside the vocabulary
+  uint32_t arrived;        // (a sequence's first row) slices weighed
 };
 
 struct VfArgs {
@@ -48,30 +55,15 @@ struct VfArgs {
   const float* probs;  // [B][T][V] or null
   const int32_t* n_draft;
   const float* u;  // [B][T + 1]
-  VfRow* rows;
+  VfRow* rows;     // [B][T + 1]
+  unsigned long long* steps;  // [B][step_stride]
   int32_t* accepted;
   int32_t* tokens;
   float* accept_prob;
   int64_t row_stride;  // of logits, elements
-  int T, V;
+  int T, V, per, step_stride;
   float inv_temp;  // 0: greedy
 };
-
-__device__ __forceinline__ uint32_t vf_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void vf_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ unsigned long long vf_peer(const unsigned long long* p, uint32_t rank) {
-  uint32_t a;
-  unsigned long long v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
-  return v;
-}
 
 // A row as 16-byte vectors: vector j holds elements j N - skew .. + N - 1, where
 // skew is the row's distance from the 16-byte boundary below it.
@@ -85,154 +77,262 @@ struct VfVec {
     count = (skew + V + N - 1) / N;
   }
   __device__ int first(int j) const { return j * N - skew; }
-  // elements outside the row read as `fill`
-  __device__ void load(int j, float (&x)[N], float fill) const {
+  // elements outside the row read as -inf
+  __device__ uint4 load(int j) const {
     const int e = first(j);
-    if (e >= 0 && e + N <= V) {
-      const uint4 w = *reinterpret_cast<const uint4*>(base + e);
-      if constexpr (sizeof(E) == 2) {
-        unpack8(w, x);
-      } else {
-        x[0] = __uint_as_float(w.x);
-        x[1] = __uint_as_float(w.y);
-        x[2] = __uint_as_float(w.z);
-        x[3] = __uint_as_float(w.w);
-      }
-    } else {
+    if (e >= 0 && e + N <= V) return *reinterpret_cast<const uint4*>(base + e);
+    uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = e + i >= 0 && e + i < V ? (float)base[e + i] : fill;
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(E) == 2) {
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(base);
+        const uint32_t lo = e + 2 * i >= 0 && e + 2 * i < V ? p[e + 2 * i] : 0xff80u;
+        const uint32_t hi = e + 2 * i + 1 >= 0 && e + 2 * i + 1 < V ? p[e + 2 * i + 1] : 0xff80u;
+        w[i] = lo | hi << 16;
+      } else {
+        w[i] = e + i >= 0 && e + i < V ? __float_as_uint(base[e + i]) : 0xff800000u;
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ static void unpack(const uint4& w, float (&x)[N]) {
+    if constexpr (sizeof(E) == 2) {
+      unpack8(w, x);
+    } else {
+      x[0] = __uint_as_float(w.x);
+      x[1] = __uint_as_float(w.y);
+      x[2] = __uint_as_float(w.z);
+      x[3] = __uint_as_float(w.w);
+    }
+  }
+  // the larger of top and a vector's elements, NaN ignored
+  __device__ static float max(const uint4& w, float top) {
+    if constexpr (sizeof(E) == 2) {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+      const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      return fmaxf(top, fmaxf(__low2float(m), __high2float(m)));
+    } else {
+      return fmaxf(fmaxf(fmaxf(top, __uint_as_float(w.x)), fmaxf(__uint_as_float(w.y), __uint_as_float(w.z))),
+                   __uint_as_float(w.w));
     }
   }
 };
 
-// floor(e 2^40) for e in [0, 1] as hi 2^20 + lo; NaN gives 0.  Adding 2^23 with
-// rounding towards zero leaves the integer part in the low mantissa bits.
-__device__ __forceinline__ void vf_fix(float e, uint32_t& hi, uint32_t& lo) {
-  e = e > 0.f ? e : 0.f;
-  const float t = e * 1048576.f;
-  const float f = __fadd_rz(t, 8388608.f);
-  hi = __float_as_uint(f) & 0x7fffffu;
-  const float r = (t - (f - 8388608.f)) * 1048576.f;
-  lo = __float_as_uint(__fadd_rz(r, 8388608.f)) & 0x7fffffu;
-}
-__device__ __forceinline__ unsigned long long vf_join(uint32_t hi, uint32_t lo) {
-  return ((unsigned long long)hi << 20) + lo;
-}
+// floor(e 2^40) for e in [0, 1], NaN as 0, without conversions: adding 8 (2^-17) with
+// rounding towards zero leaves the multiples of 2^-20 (2^-40) in the low mantissa bits.
+// hi and lo collect the raw bits of n numbers; the constants' share is taken off at the end.
+constexpr float kVfHi = 8.f, kVfLo = 0x1p-17f;
+struct VfFix {
+  uint32_t hi = 0, lo = 0, n = 0;
+  // adds one, and returns it truncated to a multiple of 2^-40
+  __device__ __forceinline__ float add(float e) {
+    e = fmaxf(e, 0.f);
+    const float f = __fadd_rz(e, kVfHi), t = f - kVfHi;
+    const float g = __fadd_rz(e - t, kVfLo);
+    hi += __float_as_uint(f);
+    lo += __float_as_uint(g);
+    ++n;
+    return t + (g - kVfLo);
+  }
+  __device__ __forceinline__ unsigned long long sum() const {
+    return ((unsigned long long)(hi - n * __float_as_uint(kVfHi)) << 20) + (lo - n * __float_as_uint(kVfLo));
+  }
+  // over the warp: 32 x 8 x 8 numbers of at most 2^20 in each part
+  __device__ __forceinline__ unsigned long long warp_sum() const {
+    const uint32_t h = __reduce_add_sync(0xffffffffu, hi - n * __float_as_uint(kVfHi));
+    const uint32_t l = __reduce_add_sync(0xffffffffu, lo - n * __float_as_uint(kVfLo));
+    return ((unsigned long long)h << 20) + l;
+  }
+};
 // The product is rounded before the subtraction (no fused multiply-add): the row's
 // maximum is the maximum of rounded products, and its own weight is exactly 2^40.
 __device__ __forceinline__ float vf_exp(float logit, float inv_temp, float mx) {
   return expf(__fsub_rn(__fmul_rn(logit, inv_temp), mx));
 }
-__device__ __forceinline__ unsigned long long vf_weight(float logit, float inv_temp, float mx) {
-  uint32_t hi, lo;
-  vf_fix(vf_exp(logit, inv_temp, mx), hi, lo);
-  return vf_join(hi, lo);
+
+// larger floats have larger keys; -inf has 0x007fffff, NaN is not asked
+__device__ __forceinline__ uint32_t vf_key(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float vf_unkey(uint32_t k) {
+  return k == 0 ? -INFINITY : __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+__device__ __forceinline__ int vf_drafts(const VfArgs& a, int b) {
+  return a.n_draft ? min(max(a.n_draft[b], 0), a.T) : a.T;
 }
 
-__device__ __forceinline__ unsigned long long vf_warp_sum(unsigned long long v) {
+// grid (slices, rows): a CTA has kVfThreads x per vectors of a row.  Rows after a
+// sequence's last draft but one are not looked at.
+template <typename E>
+__global__ void __launch_bounds__(kVfThreads) k_verify_max(VfArgs a) {
+  pdl_wait();
+  const int b = blockIdx.y / (a.T + 1), i = blockIdx.y % (a.T + 1), nd = vf_drafts(a, b);
+  if (i > nd) return;
+  const E* lg = (const E*)a.logits + (int64_t)blockIdx.y * a.row_stride;
+  VfRow* row = a.rows + blockIdx.y;
+  const VfVec<E> vec(lg, a.V);
+  float top = -INFINITY;
+  const int j0 = blockIdx.x * kVfThreads * a.per + threadIdx.x;
+  const uint32_t low = sizeof(E) == 2 ? 0xff80ff80u : 0xff800000u;
+  for (int k = 0; k < a.per; k += 4) {  // four loads in flight
+    uint4 v[4];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-// sum (or maximum) over the CTA, for every thread
-template <bool kMax>
-__device__ __forceinline__ unsigned long long vf_block(unsigned long long v, unsigned long long* sh) {
-  v = kMax ? warp_max_u64(v) : vf_warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  unsigned long long w = (threadIdx.x & 31) < kVfThreads / 32 ? sh[threadIdx.x & 31] : 0ull;
-  return kMax ? warp_max_u64(w) : vf_warp_sum(w);
+    for (int u = 0; u < 4; ++u) {
+      const int j = j0 + (k + u) * kVfThreads;
+      v[u] = k + u < a.per && j < vec.count ? vec.load(j) : make_uint4(low, low, low, low);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) top = vec.max(v[u], top);
+  }
+  const uint32_t key = __reduce_max_sync(0xffffffffu, vf_key(fmaxf(top, -INFINITY)));
+  if ((threadIdx.x & 31) == 0 && key > vf_key(-INFINITY)) atomicMax(&row->top, key);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    int drafted = 0;
+    if (i < nd) {
+      const int id = a.ids[(int64_t)b * a.T + i];
+      drafted = id >= 0 && id < a.V;
+      if (drafted) {
+        row->logit = (float)lg[id];
+        row->q = a.probs ? a.probs[((int64_t)b * a.T + i) * a.V + id] : 1.f;
+      }
+    }
+    row->drafted = drafted;
+  }
 }
 
 template <typename E>
-__global__ void __cluster_dims__(kVfCtas, 1, 1) __launch_bounds__(kVfThreads) k_verify_stats(VfArgs a) {
-  __shared__ unsigned long long sh[32];
-  __shared__ unsigned long long mine[2];
+__global__ void __launch_bounds__(kVfThreads) k_verify_sum(VfArgs a) {
   pdl_wait();
-  const uint32_t cta = vf_rank();
-  const int row = blockIdx.x / kVfCtas, b = row / (a.T + 1), i = row % (a.T + 1), tid = threadIdx.x;
-  const E* lg = (const E*)a.logits + (int64_t)row * a.row_stride;
-  const VfVec<E> vec(lg, a.V);
+  const int b = blockIdx.y / (a.T + 1), i = blockIdx.y % (a.T + 1);
+  if (i > vf_drafts(a, b)) return;
   constexpr int N = VfVec<E>::N;
-  const int per = (vec.count + kVfCtas - 1) / kVfCtas;
-  const int j0 = min((int)cta * per, vec.count), j1 = min(j0 + per, vec.count);
-  const bool greedy = a.inv_temp == 0.f;
-  const float scale = greedy ? 1.f : a.inv_temp;
-
-  unsigned long long key = 0;
-  float top = -INFINITY;
-  for (int j = j0 + tid; j < j1; j += kVfThreads) {
-    float x[N];
-    vec.load(j, x, -INFINITY);
+  VfRow* row = a.rows + blockIdx.y;
+  const VfVec<E> vec((const E*)a.logits + (int64_t)blockIdx.y * a.row_stride, a.V);
+  const float best = vf_unkey(row->top);
+  const int j0 = blockIdx.x * kVfThreads * a.per + threadIdx.x;
+  if (a.inv_temp == 0.f) {
+    if (best == -INFINITY) return;
+    uint32_t at = 0xffffffffu;
+    for (int k = 0; k < a.per; ++k) {
+      const int j = j0 + k * kVfThreads;
+      if (j >= vec.count) break;
+      float x[N];
+      vec.unpack(vec.load(j), x);
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      if (greedy) {
-        if (x[e] > top) {  // ascending indexes within a thread: the first one stays
-          top = x[e];
-          key = argmax_key(x[e], (uint32_t)(vec.first(j) + e));
+      for (int e = 0; e < N; ++e)
+        if (x[e] == best) at = min(at, (uint32_t)(vec.first(j) + e));
+    }
+    at = __reduce_min_sync(0xffffffffu, at);
+    if ((threadIdx.x & 31) == 0 && at != 0xffffffffu) atomicMax(&row->best, ~at);
+    return;
+  }
+  // rounding is monotonic: the largest product is the largest logit's
+  const float mx = __fmul_rn(best, a.inv_temp);
+  if (!(fabsf(mx) < INFINITY)) return;
+  VfFix f;
+  for (int k = 0; k < a.per; ++k) {
+    const int j = j0 + k * kVfThreads;
+    if (j >= vec.count) break;
+    float x[N];
+    vec.unpack(vec.load(j), x);
+#pragma unroll
+    for (int e = 0; e < N; ++e) f.add(vf_exp(x[e], a.inv_temp, mx));
+  }
+  const unsigned long long s = f.warp_sum();
+  if ((threadIdx.x & 31) == 0 && s) atomicAdd(&row->sum, s);
+}
+
+// What a sequence's rows say: drafts accepted, and the row the next token is drawn from.
+struct VfSeq {
+  const VfRow* row;
+  int accepted;
+  bool refused;
+};
+// By a whole warp, lane i for draft i; prob: lane i's min(1, p / q).
+__device__ __forceinline__ VfSeq vf_decide(const VfArgs& a, int b, float* prob) {
+  const int lane = threadIdx.x & 31, nd = vf_drafts(a, b);
+  const VfRow* rows = a.rows + (int64_t)b * (a.T + 1);
+  bool ok = false;
+  *prob = 0.f;
+  if (lane < nd) {
+    const VfRow r = rows[lane];
+    if (r.drafted) {
+      if (a.inv_temp == 0.f) {
+        ok = r.best != 0 && (int)~r.best == a.ids[(int64_t)b * a.T + lane];
+        *prob = ok ? 1.f : 0.f;
+      } else {
+        VfFix f;
+        const float w = f.add(vf_exp(r.logit, a.inv_temp, __fmul_rn(vf_unkey(r.top), a.inv_temp)));
+        const float p = r.sum ? __fdiv_rn(w, (float)r.sum * 0x1p-40f) : 0.f;
+        ok = __fmul_rn(a.u[(int64_t)b * (a.T + 1) + lane], r.q) < p;
+        *prob = r.q > 0.f ? fminf(__fdiv_rn(p, r.q), 1.f) : p > 0.f ? 1.f : 0.f;
+      }
+    }
+  }
+  VfSeq s;
+  s.accepted = __ffs((int)__ballot_sync(0xffffffffu, !ok)) - 1;  // nd <= 31: lane nd has none
+  s.refused = s.accepted < nd;
+  s.row = rows + s.accepted;
+  return s;
+}
+
+// The weights of the row that a token is drawn from.
+template <typename E>
+struct VfDraw {
+  static constexpr int N = VfVec<E>::N;
+  VfVec<E> vec;
+  const float* q;
+  bool q_vec, residual;
+  int id;
+  float z, mx, inv_temp;
+  __device__ VfDraw(const VfArgs& a, int b, const VfSeq& s)
+      : vec((const E*)a.logits + ((int64_t)b * (a.T + 1) + s.accepted) * a.row_stride, a.V) {
+    residual = s.refused;
+    id = s.refused ? a.ids[(int64_t)b * a.T + s.accepted] : -1;
+    q = s.refused && a.probs ? a.probs + ((int64_t)b * a.T + s.accepted) * a.V : nullptr;
+    q_vec = ((reinterpret_cast<uintptr_t>(q) - vec.skew * 4) & 15u) == 0;
+    z = (float)s.row->sum * 0x1p-40f;
+    inv_temp = a.inv_temp;
+    mx = __fmul_rn(vf_unkey(s.row->top), a.inv_temp);
+  }
+  // adds the weights of vector j to f; `each`: the running sums after every element
+  __device__ __forceinline__ void weigh(int j, VfFix& f, unsigned long long* each) const {
+    float x[N], d[N];
+    vec.unpack(vec.load(j), x);
+    const int v0 = vec.first(j);
+    if (residual && q) {
+      if (q_vec && v0 >= 0 && v0 + N <= vec.V) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+          const float4 y = *reinterpret_cast<const float4*>(q + v0 + e);
+          d[e] = y.x;
+          d[e + 1] = y.y;
+          d[e + 2] = y.z;
+          d[e + 3] = y.w;
         }
       } else {
-        top = fmaxf(top, __fmul_rn(x[e], scale));  // (ignores NaN)
-      }
-    }
-  }
-  if (!greedy) key = argmax_key(top, 0u);
-  key = vf_block<true>(key, sh);
-  if (tid == 0) mine[0] = key;
-  vf_sync();
-  for (int r = 0; r < kVfCtas; ++r) {
-    const unsigned long long k = vf_peer(&mine[0], r);
-    key = k > key ? k : key;
-  }
-  const uint32_t ord = (uint32_t)(key >> 32);
-  const float mx = key == 0 ? -INFINITY : __uint_as_float((ord & 0x80000000u) ? (ord & 0x7fffffffu) : ~ord);
-  VfRow out = {0ull, mx, -1, 0, 0};
-  if (greedy) {
-    if (key != 0) out.best = (int)argmax_key_index(key);
-  } else if (fabsf(mx) < INFINITY) {
-    uint32_t hi = 0, lo = 0;  // at most 2^20 / 4096 elements per thread: 2^28 each
-    for (int j = j0 + tid; j < j1; j += kVfThreads) {
-      float x[N];
-      vec.load(j, x, -INFINITY);
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        uint32_t h, l;
-        vf_fix(vf_exp(x[e], scale, mx), h, l);
-        hi += h;
-        lo += l;
+        for (int e = 0; e < N; ++e) d[e] = v0 + e >= 0 && v0 + e < vec.V ? q[v0 + e] : 0.f;
       }
     }
-    const unsigned long long s = vf_block<false>(vf_join(hi, lo), sh);
-    if (tid == 0) mine[1] = s;
-  }
-  if (tid == 0 && (greedy || !(fabsf(mx) < INFINITY))) mine[1] = 0;
-  vf_sync();
-  if (cta == 0 && tid == 0) {
-    for (int r = 0; r < kVfCtas; ++r) out.sum += vf_peer(&mine[1], r);
-    if (i < a.T) {
-      const int n = a.n_draft ? min(max(a.n_draft[b], 0), a.T) : a.T;
-      float prob = 0.f;
-      if (i < n) {
-        const int id = a.ids[(int64_t)b * a.T + i];
-        if (id >= 0 && id < a.V) {
-          if (greedy) {
-            out.ok = id == out.best;
-            prob = out.ok ? 1.f : 0.f;
-          } else {
-            const float p = out.sum ? __fdiv_rn((float)vf_weight((float)lg[id], scale, mx), (float)out.sum) : 0.f;
-            const float q = a.probs ? a.probs[((int64_t)b * a.T + i) * a.V + id] : 1.f;
-            out.ok = __fmul_rn(a.u[(int64_t)b * (a.T + 1) + i], q) < p;
-            prob = q > 0.f ? fminf(__fdiv_rn(p, q), 1.f) : p > 0.f ? 1.f : 0.f;
-          }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      float y = vf_exp(x[e], inv_temp, mx);
+      if (residual) {
+        if (!q) {
+          if (v0 + e == id) y = 0.f;
+        } else {
+          VfFix one;
+          const float p = __fdiv_rn(one.add(y), z);
+          y = p > d[e] ? p - d[e] : 0.f;
         }
       }
-      a.accept_prob[(int64_t)b * a.T + i] = prob;
+      f.add(y);
+      if (each) each[e] = f.sum();
     }
-    a.rows[row] = out;
   }
-  vf_sync();  // no CTA leaves while its shared memory may be read
-}
+};
 
 // floor(total u) with u taken to 24 bits; total < 2^63
 __device__ __forceinline__ unsigned long long vf_threshold(unsigned long long total, float u) {
@@ -241,137 +341,157 @@ __device__ __forceinline__ unsigned long long vf_threshold(unsigned long long to
   const unsigned long long f = (unsigned long long)t;
   return (total >> 32) * f * 256ull + (((total & 0xffffffffull) * f) >> 24);
 }
-
-template <typename E>
-__global__ void __cluster_dims__(kVfCtas, 1, 1) __launch_bounds__(kVfThreads) k_verify_draw(VfArgs a) {
-  __shared__ unsigned long long sh[32];
-  __shared__ unsigned long long mine[2];
-  __shared__ int found;
-  pdl_wait();
-  const uint32_t cta = vf_rank();
-  const int b = blockIdx.x / kVfCtas, tid = threadIdx.x, lane = tid & 31;
-  const int T = a.T;
-  const int nd = a.n_draft ? min(max(a.n_draft[b], 0), T) : T;
-  const VfRow* rows = a.rows + (int64_t)b * (T + 1);
-  const uint32_t no = __ballot_sync(0xffffffffu, lane >= nd || !rows[min(lane, T)].ok);
-  const int n = __ffs((int)no) - 1;  // nd <= 31, so a bit is set
-  const VfRow row = rows[n];
-  const bool greedy = a.inv_temp == 0.f;
-  int extra = greedy ? row.best : -1;
-
-  if (!greedy && row.sum != 0) {
-    const E* lg = (const E*)a.logits + ((int64_t)b * (T + 1) + n) * a.row_stride;
-    const VfVec<E> vec(lg, a.V);
-    constexpr int N = VfVec<E>::N;
-    const int per = (vec.count + kVfCtas - 1) / kVfCtas;
-    const int j0 = min((int)cta * per, vec.count), j1 = min(j0 + per, vec.count);
-    const bool refused = n < nd;
-    const int id = refused ? a.ids[(int64_t)b * T + n] : -1;
-    const float* q = refused && a.probs ? a.probs + ((int64_t)b * T + n) * a.V : nullptr;
-    const float z = (float)row.sum;
-    bool residual = refused;
-    auto weights = [&](int j, unsigned long long (&w)[N]) {
-      float x[N];
-      vec.load(j, x, -INFINITY);
+__device__ __forceinline__ unsigned long long vf_scan(unsigned long long x) {  // inclusive, over a warp
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int v = vec.first(j) + e;
-        w[e] = vf_weight(x[e], a.inv_temp, row.max);
-        if (residual) {
-          if (!q) {
-            if (v == id) w[e] = 0;
-          } else if (v >= 0 && v < a.V) {
-            const float p = __fdiv_rn((float)w[e], z), d = q[v];
-            uint32_t hi, lo;
-            vf_fix(p > d ? p - d : 0.f, hi, lo);
-            w[e] = vf_join(hi, lo);
-          }
-        }
-      }
-    };
-    unsigned long long total, before;
-    for (int pass = 0;; ++pass) {
-      unsigned long long s = 0;
-      for (int j = j0 + tid; j < j1; j += kVfThreads) {
-        unsigned long long w[N];
-        weights(j, w);
-#pragma unroll
-        for (int e = 0; e < N; ++e) s += w[e];
-      }
-      s = vf_block<false>(s, sh);
-      if (tid == 0) mine[pass] = s;
-      vf_sync();
-      total = before = 0;
-      for (int r = 0; r < kVfCtas; ++r) {
-        const unsigned long long x = vf_peer(&mine[pass], r);
-        if (r < (int)cta) before += x;
-        total += x;
-      }
-      if (total != 0 || !residual) break;
-      residual = false;  // p nowhere above q (rounding): the target's own distribution
-    }
-    const unsigned long long k = vf_threshold(total, a.u[(int64_t)b * (T + 1) + T]);
-    // the CTA whose slice holds the running sum's crossing looks for it, 512 vectors at a time
-    if (tid == 0) found = -1;
-    __syncthreads();
-    if (k >= before) {
-      unsigned long long run = before;
-      for (int js = j0; js < j1; js += kVfThreads) {
-        const int j = js + tid;
-        unsigned long long w[N], s = 0;
-        if (j < j1) {
-          weights(j, w);
-#pragma unroll
-          for (int e = 0; e < N; ++e) s += w[e];
-        }
-        // inclusive scan over the CTA
-        unsigned long long x = s;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
-          if (lane >= o) x += y;
-        }
-        __syncthreads();
-        if (lane == 31) sh[tid >> 5] = x;
-        __syncthreads();
-        unsigned long long low = run, all = run;
-        for (int r = 0; r < kVfThreads / 32; ++r) {
-          if (r < (tid >> 5)) low += sh[r];
-          all += sh[r];
-        }
-        const unsigned long long hi_ = low + x, lo_ = hi_ - s;
-        if (j < j1 && lo_ <= k && k < hi_) {
-          unsigned long long c = lo_;
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            if (c <= k && k < c + w[e]) found = vec.first(j) + e;
-            c += w[e];
-          }
-        }
-        if (all > k) break;
-        run = all;
-      }
-    }
-    __syncthreads();
-    extra = found;
-    vf_sync();  // peers have read this CTA's sums
-    if (extra < 0) return;  // another CTA has the token
-  } else if (cta != 0) {
-    return;
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
   }
+  return x;
+}
+
+// By one CTA per sequence: the draw, the outputs, and the rows' records zero again.
+template <typename E>
+__device__ __forceinline__ void vf_pick(const VfArgs& a, int b, const VfSeq& s, float prob, float u) {
+  __shared__ unsigned long long warps[kVfWarps], reached;
+  __shared__ int token;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, T = a.T;
+  if (tid < T) a.accept_prob[(int64_t)b * T + tid] = prob;
+  if (tid == 0) {
+    a.accepted[b] = s.accepted;
+    token = a.inv_temp == 0.f && s.row->best != 0 ? (int)~s.row->best : -1;
+  }
+  if (a.inv_temp != 0.f && s.row->sum != 0) {
+    VfDraw<E> draw(a, b, s);
+    constexpr int N = VfDraw<E>::N;
+    unsigned long long* steps = a.steps + (int64_t)b * a.step_stride;
+    const int n = (draw.vec.count + 31) / 32, per = (n + kVfThreads - 1) / kVfThreads;
+    unsigned long long mine, before, total;
+    for (;;) {
+      // thread t has steps [t per, (t + 1) per)
+      mine = 0;
+#pragma unroll 4
+      for (int k = tid * per; k < min(n, (tid + 1) * per); ++k) mine += __ldcg(steps + k);
+      const unsigned long long x = vf_scan(mine);
+      if (lane == 31) warps[warp] = x;
+      __syncthreads();
+      before = x - mine;
+      total = 0;
+#pragma unroll
+      for (int w = 0; w < kVfWarps; ++w) {
+        if (w < warp) before += warps[w];
+        total += warps[w];
+      }
+      if (total != 0 || !draw.residual) break;
+      // p nowhere above q (rounding): the target's own distribution, weighed here
+      draw.residual = false;
+      __syncthreads();
+      for (int k = warp; k < n; k += kVfWarps) {
+        VfFix f;
+        if (k * 32 + lane < draw.vec.count) draw.weigh(k * 32 + lane, f, nullptr);
+        const unsigned long long y = f.warp_sum();
+        if (lane == 0) steps[k] = y;
+      }
+      __syncthreads();
+    }
+    const unsigned long long at = vf_threshold(total, u);
+    if (before <= at && at < before + mine) {  // one thread: its step with the crossing
+      int k = tid * per;
+      for (unsigned long long x; before + (x = steps[k]) <= at; ++k) before += x;
+      reached = before;
+      token = k;
+    }
+    __syncthreads();
+    const int j = token * 32 + lane;
+    before = reached;
+    __syncthreads();
+    if (warp == 0) {
+      unsigned long long each[N], sum = 0;
+      VfFix f;
+      if (j < draw.vec.count) {
+        draw.weigh(j, f, each);
+        sum = f.sum();
+      }
+      const unsigned long long upto = before + vf_scan(sum);
+      if (upto - sum <= at && at < upto) {
+        int e = 0;
+        while (upto - sum + each[e] <= at) ++e;
+        token = draw.vec.first(j) + e;
+      }
+    }
+  }
+  __syncthreads();
   if (tid <= T) {
     int t = -1;
-    if (tid < n) t = a.ids[(int64_t)b * T + tid];
-    if (tid == n) t = extra;
+    if (tid < s.accepted) t = a.ids[(int64_t)b * T + tid];
+    if (tid == s.accepted) t = token;
     a.tokens[(int64_t)b * (T + 1) + tid] = t;
+    VfRow* r = a.rows + (int64_t)b * (T + 1) + tid;
+    r->sum = 0;
+    r->top = r->best = r->arrived = 0;
   }
-  if (tid == 0) a.accepted[b] = n;
+}
+
+// grid (slices, sequences): the weights' sums of every step (32 vectors, a warp); the last
+// CTA of a sequence to arrive draws its token
+template <typename E>
+__global__ void __launch_bounds__(kVfThreads) k_verify_weigh(VfArgs a) {
+  __shared__ bool last;
+  pdl_wait();
+  const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float u = a.u[(int64_t)b * (a.T + 1) + a.T];
+  float prob;
+  const VfSeq s = vf_decide(a, b, &prob);
+  if (s.row->sum != 0) {
+    const VfDraw<E> draw(a, b, s);
+    for (int k = 0; k < a.per; ++k) {
+      const int step = (blockIdx.x * a.per + k) * kVfWarps + warp, j = step * 32 + lane;
+      if (step * 32 >= draw.vec.count) break;
+      VfFix f;
+      if (j < draw.vec.count) draw.weigh(j, f, nullptr);
+      const unsigned long long x = f.warp_sum();
+      if (lane == 0) a.steps[(int64_t)b * a.step_stride + step] = x;
+    }
+  }
+  if (lane == 0) __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(&a.rows[(int64_t)b * (a.T + 1)].arrived, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  vf_pick<E>(a, b, s, prob, u);
+}
+
+// temperature 0: nothing to weigh
+template <typename E>
+__global__ void __launch_bounds__(kVfThreads) k_verify_greedy(VfArgs a) {
+  pdl_wait();
+  float prob;
+  const VfSeq s = vf_decide(a, blockIdx.x, &prob);
+  vf_pick<E>(a, blockIdx.x, s, prob, 0.f);
 }
 
 template <typename E>
-static int verify_launch(const VfArgs& a, int B, cudaStream_t s) {
-  JSX_CUDA(launch_kernel(k_verify_stats<E>, dim3((unsigned)(B * (a.T + 1) * kVfCtas)), dim3(kVfThreads), 0, s, a));
-  JSX_CUDA(launch_kernel(k_verify_draw<E>, dim3((unsigned)(B * kVfCtas)), dim3(kVfThreads), 0, s, a));
+static int verify_launch(VfArgs& a, int B, cudaStream_t s) {
+  // eight CTAs per SM (a full one) where the rows suffice: more, shorter ones cost more to
+  // launch than they even out (32 x 5 rows of 151552: 12.7 us for the maxima, 20.9 us at one vector a thread)
+  const int most = (a.V + 2 * VfVec<E>::N - 2) / VfVec<E>::N;  // vectors of a row, wherever it begins
+  auto cut = [&](int rows) {
+    const int64_t units = (int64_t)rows * ((most + kVfThreads - 1) / kVfThreads);
+    const int64_t per = (units + 8ll * sm_count() - 1) / (8ll * sm_count());
+    a.per = (int)(per < 1 ? 1 : per > kVfMaxPer ? kVfMaxPer : per);
+    return (unsigned)((most + kVfThreads * a.per - 1) / (kVfThreads * a.per));
+  };
+  const unsigned slices = cut(B * (a.T + 1));
+  JSX_CUDA(launch_kernel(k_verify_max<E>, dim3(slices, B * (a.T + 1)), dim3(kVfThreads), 0, s, a));
+  JSX_CUDA(launch_kernel(k_verify_sum<E>, dim3(slices, B * (a.T + 1)), dim3(kVfThreads), 0, s, a));
+  if (a.inv_temp != 0.f) {
+    const unsigned n = cut(B);
+    JSX_CUDA(launch_kernel(k_verify_weigh<E>, dim3(n, B), dim3(kVfThreads), 0, s, a));
+  } else {
+    JSX_CUDA(launch_kernel(k_verify_greedy<E>, dim3(B), dim3(kVfThreads), 0, s, a));
+  }
   return JSX_OK;
 }
 
@@ -379,9 +499,12 @@ static int verify_launch(const VfArgs& a, int B, cudaStream_t s) {
 
 using namespace jsx;
 
+// steps of a row: the 32-bit form has the most
+static int64_t vf_steps(int V) { return (V + 6) / 4 / 32 + 1; }
+
 extern "C" int jsx_verify_workspace_size(int B, int T, int V, size_t* bytes) {
   JSX_REQUIRE(bytes && B >= 1 && T >= 0 && T <= kVfMaxDraft && V >= 1 && V <= kVfMaxVocab, "bad arguments");
-  *bytes = (size_t)B * (T + 1) * sizeof(VfRow);
+  *bytes = (size_t)B * (T + 1) * sizeof(VfRow) + (size_t)B * vf_steps(V) * 8;
   return JSX_OK;
 }
 
@@ -389,7 +512,8 @@ extern "C" int jsx_verify_drafts(const void* logits, int logits_f32, int64_t row
                                  const float* draft_probs, const int32_t* n_draft, const float* uniforms,
                                  float temperature, int32_t* accepted, int32_t* tokens, float* accept_prob, int B,
                                  int T, int V, void* workspace, size_t workspace_bytes, void* stream) {
-  JSX_REQUIRE(B >= 1 && B <= (1 << 20) && T >= 0 && T <= kVfMaxDraft, "B=%d T=%d (T in 0..%d)", B, T, kVfMaxDraft);
+  JSX_REQUIRE(B >= 1 && T >= 0 && T <= kVfMaxDraft && (int64_t)B * (T + 1) <= 65535, "B=%d T=%d (T in 0..%d, B (T + 1) up to 65535)", B,
+              T, kVfMaxDraft);
   JSX_REQUIRE(V >= 1 && V <= kVfMaxVocab && row_stride >= V, "V=%d (1..%d) row_stride=%lld", V, kVfMaxVocab,
               (long long)row_stride);
   JSX_REQUIRE(logits && accepted && tokens, "null pointer argument");
@@ -409,6 +533,8 @@ extern "C" int jsx_verify_drafts(const void* logits, int logits_f32, int64_t row
   a.n_draft = n_draft;
   a.u = uniforms;
   a.rows = (VfRow*)workspace;
+  a.steps = (unsigned long long*)((char*)workspace + (size_t)B * (T + 1) * sizeof(VfRow));
+  a.step_stride = (int)vf_steps(V);
   a.accepted = accepted;
   a.tokens = tokens;
   a.accept_prob = accept_prob;

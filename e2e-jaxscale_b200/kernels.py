@@ -679,7 +679,7 @@ def pages_compact(table, held, refs, pool, workspace, table_out=None, refs_out=N
 def verify_workspace(B, T, V, device) -> torch.Tensor:
     n = ctypes.c_size_t(0)
     call("jsx_verify_workspace_size", B, T, V, ctypes.byref(n))
-    return torch.empty(n.value, dtype=torch.uint8, device=device)
+    return torch.zeros(n.value, dtype=torch.uint8, device=device)
 
 
 def verify_drafts(logits, draft_ids, uniforms, workspace, draft_probs=None, n_draft=None, temperature=1.0,

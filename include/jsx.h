@@ -500,7 +500,9 @@ int jsx_pages_compact(const int32_t* table, const int32_t* held, const int32_t* 
  * ids outside [0, V).  temperature 0: greedy (p = 1 at the first maximum; uniforms
  * may be NULL).  Sums are over integers (weights of 2^-40), so the tokens do not
  * depend on the order of execution.  NaN logits have no mass; a row without a
- * finite maximum accepts nothing and draws -1.  0 <= T <= 31, V <= 2^20. */
+ * finite maximum accepts nothing and draws -1.  0 <= T <= 31, V <= 2^20,
+ * B (T + 1) <= 65535.  workspace: jsx_verify_workspace_size bytes, 16-byte aligned,
+ * zero-filled once (left so that the next call can use it). */
 int jsx_verify_workspace_size(int B, int T, int V, size_t* bytes);
 int jsx_verify_drafts(const void* logits, int logits_f32, int64_t row_stride,
                       const int32_t* draft_ids, const float* draft_probs, const int32_t* n_draft,
