@@ -40,7 +40,7 @@ constexpr int kKaKeys = kKaChunk / kKaWarps;
 constexpr int kKaPieces = kKaKeys / 16;
 constexpr int kKaThreads = (kKaWarps + 1) * 32;  // and one that copies
 constexpr int kKaPerSm = 2;     // CTAs per SM (three of 128 registers a thread measured slower: 73 against 70 us)
-constexpr int kKaStages = 4;
+constexpr int kKaStages = 3;
 constexpr int kKaFan = 16;      // parts joined at once
 constexpr int kKaLevels = 3;    // 16^3 parts of an item at most
 constexpr int kKaListMax = 512;   // (sequence, row tile) pairs up to which the chunk list is cut into ranges
@@ -69,7 +69,7 @@ struct KaArgs {
   int num_pages, slots, B, T, nkv, G, tiles, pt, pt_log, window, sinks;
   uint32_t per_g;  // 2^32 / G rounded up: x / G = umulhi(x, per_g) for x G < 2^32 (G > 1)
   int listed;  // chunk list cut into ranges; else whole items per CTA
-  uint32_t negate;   // 0x80000000 when the scale is negative
+  int negate;        // the scale is negative
   float scale_log2;  // its magnitude x log2(e)
 };
 
@@ -77,6 +77,7 @@ template <int D>
 struct KaShape {
   static constexpr int kStage = kv4_block_bytes(kKaChunk, D);
   static constexpr int kRecord = kKaRows * D + 2 * kKaRows;  // floats: output, maxima, sums
+  static constexpr int kQRow = D * 2 + 16;                   // bytes: rows' pieces in different banks
 };
 
 __device__ __forceinline__ int ka_div_g(const KaArgs& a, int x) { return a.G == 1 ? x : (int)__umulhi((uint32_t)x, a.per_g); }
@@ -170,13 +171,13 @@ __device__ __forceinline__ KaPos ka_first(const KaArgs& a, int* cum, int lane) {
     return q;
   }
   uint32_t total = 0;
+#pragma unroll 2
   for (int b0 = 0; b0 < a.B; b0 += 32) {
     const int b = b0 + lane;
     int n = 0;
     if (b < a.B)
       for (int t = 0; t < a.tiles; ++t) n += ka_tile(a, b, t).n;
-    n *= a.nkv;
-    int v = n;
+    int v = n * a.nkv;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, v, o);
@@ -198,16 +199,25 @@ __device__ __forceinline__ KaPos ka_first(const KaArgs& a, int* cum, int lane) {
   int n = 0;  // sequences whose chunks begin at or before w: the last of them is it
   for (int b0 = 0; b0 < a.B; b0 += 32) n += __popc(__ballot_sync(0xffffffffu, b0 + lane < a.B && cum[b0 + lane] <= q.w));
   q.b = n - 1;
-  int off = q.w - cum[q.b], per = 0;
-  for (int t = 0; t < a.tiles; ++t) per += ka_tile(a, q.b, t).n;
-  while (off >= per) {
-    off -= per;
-    ++q.h;
-  }
-  for (;; ++q.tile) {
-    q.x = ka_tile(a, q.b, q.tile);
-    if (off < q.x.n) break;
-    off -= q.x.n;
+  int off = q.w - cum[q.b];
+  if (a.tiles == 1) {
+    q.x = ka_tile(a, q.b, 0);
+    while (off >= q.x.n) {
+      off -= q.x.n;
+      ++q.h;
+    }
+  } else {
+    int per = 0;
+    for (int t = 0; t < a.tiles; ++t) per += ka_tile(a, q.b, t).n;
+    while (off >= per) {
+      off -= per;
+      ++q.h;
+    }
+    for (;; ++q.tile) {
+      q.x = ka_tile(a, q.b, q.tile);
+      if (off < q.x.n) break;
+      off -= q.x.n;
+    }
   }
   q.c0 = off;
   q.c1 = min(q.x.n, off + q.w1 - q.w);
@@ -270,31 +280,13 @@ __device__ __forceinline__ bool ka_wait(uint64_t* b, uint32_t parity, volatile u
 }
 __device__ __forceinline__ bool ka_nan_scale(uint32_t s) { return (s & 0x7fu) == 0x7fu; }
 
-// One row's D / 4 values of q at `p` as f16 pairs, scaled by the power of two that brings
-// the row's largest magnitude to 2^8 .. 2^9; returns what undoes it.
-template <int N>
-__device__ __forceinline__ float ka_load_q(const bf16* p, bool live, uint32_t (&h)[N / 2], uint32_t negate) {
-  uint32_t w[N / 2];
-#pragma unroll
-  for (int i = 0; i < N / 8; ++i) {
-    const uint4 v = live ? *reinterpret_cast<const uint4*>(p + 8 * i) : make_uint4(0, 0, 0, 0);
-    w[4 * i] = v.x;
-    w[4 * i + 1] = v.y;
-    w[4 * i + 2] = v.z;
-    w[4 * i + 3] = v.w;
-  }
-  uint32_t mx = 0;
-#pragma unroll
-  for (int i = 0; i < N / 2; ++i) mx = __vmaxu2(mx, w[i] & 0x7fff7fffu);
-  uint32_t top = max(mx & 0xffffu, mx >> 16);
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+// The power of two that brings a row of q, whose largest magnitude has the bf16 bits `top`,
+// to 2^8 .. 2^9, and the one that undoes it.
+__device__ __forceinline__ float ka_q_scale(uint32_t top, float* undo) {
   const int e = (int)(top >> 7);  // exponent field of the largest
   const int f = e == 255 ? 127 : min(262 - e, 254);
-  const float mul = __uint_as_float((uint32_t)f << 23 | negate);
-#pragma unroll
-  for (int i = 0; i < N / 2; ++i) h[i] = ka_h2(bf_lo(w[i]) * mul, bf_hi(w[i]) * mul);
-  return f == 254 ? 0x1p-127f : __uint_as_float((uint32_t)(254 - f) << 23);
+  *undo = f == 254 ? 0x1p-127f : __uint_as_float((uint32_t)(254 - f) << 23);
+  return __uint_as_float((uint32_t)f << 23);
 }
 
 // Four values of a row's result; `l` is the weights' sum.
@@ -310,16 +302,17 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
   constexpr int NV = D / 8;       // n tiles of O = dimensions per column
   constexpr int VW = D / 64;      // words of codes per lane and V row
   extern __shared__ __align__(128) unsigned char ring[];
-  __shared__ __align__(16) float join[kKaWarps * kKaRows * D];  // the warps' outputs; before that q as MMA operands [D / 16][32 lanes]
-  __shared__ float join_m[kKaWarps * kKaRows], join_l[kKaWarps * kKaRows];
+  __shared__ __align__(16) float join[kKaWarps * kKaRows * D];  // the warps' outputs
+  __shared__ __align__(16) float join_m[kKaRows * kKaWarps], join_l[kKaRows * kKaWarps];
+  __shared__ __align__(16) unsigned char qrow[2][kKaRows * S::kQRow];  // q's rows of this item and the next
+  __shared__ uint4 qfrag[D / 16 * 32];                                 // q as MMA operands
+  __shared__ __align__(16) uint32_t q_top[kKaRows * kKaWarps];         // rows' largest magnitudes, per quarter
   __shared__ int cum[kKaListMax + 1];
-  __shared__ KaPos place[2];
-  __shared__ uint64_t full[kKaStages], empty[kKaStages];
+  __shared__ KaPos place[2];  // this item and the next, as the copying warp finds them
+  __shared__ uint64_t full[kKaStages], empty[kKaStages], begun[2], ended[2];
   __shared__ uint32_t present[kKaStages];  // pages of the stage that were copied
   __shared__ uint32_t flags[2];            // [0] a wait gave up, [1] last to arrive
-  __shared__ int row_token[kKaRows], row_head[kKaRows];
   __shared__ float* recs[kKaFan];
-  uint4* qfrag = reinterpret_cast<uint4*>(join);
   volatile uint32_t* abort = flags;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
@@ -328,31 +321,44 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
       tc_mbar_init(&full[s], 1);
       tc_mbar_init(&empty[s], kKaWarps);
     }
+    for (int s = 0; s < 2; ++s) {
+      tc_mbar_init(&begun[s], 1);
+      tc_mbar_init(&ended[s], kKaWarps);
+    }
     flags[0] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  pdl_wait();
-  if (warp == kKaWarps) {
-    const KaPos q = ka_first(a, cum, lane);
-    if (lane == 0) place[0] = place[1] = q;
-  }
   __syncthreads();
+  pdl_wait();
   const uint32_t block = kv4_block_bytes(a.pt, D);
 
   if (warp == kKaWarps) {
-    // ---- copies: a lane per page of the chunk, a whole page's block at once ----
-    KaPos& p = place[1];
+    // ---- places, q's rows and pages: the copying warp runs ahead of the others ----
     const int pages = kKaChunk >> a.pt_log;
-    uint32_t f = 0;
-    while (p.live) {
+    uint32_t f = 0, k = 0;
+    KaPos first = ka_first(a, cum, lane);
+    if (lane == 0) place[0] = first;
+    __syncwarp();
+    for (;; ++k) {
+      KaPos& p = place[k & 1];
+      // q's rows: a lane each
+      const int row = p.tile * kKaRows + lane, i = ka_div_g(a, row);
+      const bool q_on = p.live && lane < kKaRows && row < a.G * a.T;
+      const uint32_t q_rows = __popc(__ballot_sync(0xffffffffu, q_on));
+      if (lane == 0) tc_expect_tx(&begun[k & 1], q_rows * D * 2);
+      __syncwarp();
+      if (q_on)
+        ka_copy(&qrow[k & 1][lane * S::kQRow],
+                a.q + ((int64_t)p.b * a.T + i) * a.q_stride + (int64_t)(p.h * a.G + row - i * a.G) * D, D * 2, &begun[k & 1]);
+      if (!p.live) break;
       const int c0 = p.c0, c1 = p.c1, lo_chunk = p.x.lo_chunk, sink_chunks = p.x.sink_chunks, hi = p.x.hi;
       const int sinks = min(a.sinks, hi);
-      const int32_t* row = a.table + (int64_t)p.b * a.slots;
+      const int32_t* table = a.table + (int64_t)p.b * a.slots;
       const int64_t head = p.h;
       auto look_up = [&](int c) {
         const int chunk = c < sink_chunks ? c : lo_chunk + c - sink_chunks;
         const int slot = chunk * pages + lane;
-        return lane < pages && (slot << a.pt_log) < (c < sink_chunks ? sinks : hi) && slot < a.slots ? row[slot] : -1;
+        return lane < pages && (slot << a.pt_log) < (c < sink_chunks ? sinks : hi) && slot < a.slots ? table[slot] : -1;
       };
       int soon = c0 < c1 ? look_up(c0) : -1;  // pages are looked up a chunk ahead
       for (int c = c0; c < c1; ++c, ++f) {
@@ -370,14 +376,18 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
         if (have >> lane & 1u)
           ka_copy(ring + s * S::kStage + lane * block, a.pool + ((int64_t)page * a.nkv + head) * block, block, &full[s]);
       }
-      __syncwarp();
-      if (lane == 0) ka_next(a, cum, &p);
+      if (k >= 1 && !ka_wait(&ended[(k + 1) & 1], ((k + 1) / 2 - 1) & 1, abort)) goto landed;
+      if (lane == 0) {
+        place[(k + 1) & 1] = p;
+        ka_next(a, cum, &place[(k + 1) & 1]);
+      }
       __syncwarp();
     }
   landed:
     // the copies in flight land before this CTA's shared memory is given away, also when a wait gave up
-    for (uint32_t k = f > kKaStages ? f - kKaStages : 0; k < f; ++k)
-      tc_wait_err(&full[k % kKaStages], (k / kKaStages) & 1, nullptr, &g_kv4_error);
+    for (uint32_t x = f > kKaStages ? f - kKaStages : 0; x < f; ++x)
+      tc_wait_err(&full[x % kKaStages], (x / kKaStages) & 1, nullptr, &g_kv4_error);
+    for (uint32_t x = k > 0 ? k - 1 : 0; x <= k; ++x) tc_wait_err(&begun[x & 1], (x / 2) & 1, nullptr, &g_kv4_error);
     return;
   }
 
@@ -398,31 +408,53 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
   }
   bool bad = false;
   uint32_t stage = 0, phase = 0;
-  KaPos& it = place[0];
-  while (it.live) {
-      if (tid < kKaRows) {
-        const int row = it.tile * kKaRows + tid, i = ka_div_g(a, row);
-        row_token[tid] = row < a.G * a.T ? i : -1;
-        row_head[tid] = it.h * a.G + row - i * a.G;
-      }
-      ka_sync();
+  for (uint32_t item = 0;; ++item) {
+      // (a wait that gave up in one warp ends the loop in all)
+      if (!epi_all(ka_wait(&begun[item & 1], (item / 2) & 1, abort))) break;
+      const KaPos& it = place[item & 1];
+      if (!it.live) break;
+      // q as MMA operands: each warp converts its quarter of the dimensions, after the rows'
+      // largest magnitudes have met in shared memory
+      constexpr int QW = D / 32;  // words of two values per lane and row
       float sc[2];
       int rowpos[2];
+      uint32_t qv[2][QW];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int i = row_token[g + 8 * k];
-        const bf16* p = a.q + ((int64_t)it.b * a.T + i) * a.q_stride + row_head[g + 8 * k] * D + t * (D / 4);
-        uint32_t h[D / 8];
-        sc[k] = fmaxf(a.scale_log2 * ka_load_q<D / 4>(p, i >= 0, h, a.negate), 1e-37f);  // never 0: 0 x -inf
-        // (every warp needs every row's scale; each writes a quarter of the operands)
+        const int r = g + 8 * k, row = it.tile * kKaRows + r;
+        const bool live = row < a.G * a.T;
+        const uint32_t at = s_u32(&qrow[item & 1][r * S::kQRow]) + t * (D / 2) + warp * (D / 8);
+        if constexpr (D == 128) {
+          const uint4 v = ka_lds128(at);
+          qv[k][0] = v.x, qv[k][1] = v.y, qv[k][2] = v.z, qv[k][3] = v.w;
+        } else {
+          const uint2 v = ka_lds64(at);
+          qv[k][0] = v.x, qv[k][1] = v.y;
+        }
+        uint32_t mx = 0;
+#pragma unroll
+        for (int i = 0; i < QW; ++i) {
+          qv[k][i] = live ? qv[k][i] : 0u;
+          mx = __vmaxu2(mx, qv[k][i] & 0x7fff7fffu);
+        }
+        mx = max(mx & 0xffffu, mx >> 16);
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        if (t == 0) q_top[r * kKaWarps + warp] = mx;
+        rowpos[k] = it.x.pos + (live ? ka_div_g(a, row) : 0);
+      }
+      ka_sync();
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint4 tops = *reinterpret_cast<const uint4*>(q_top + (g + 8 * k) * kKaWarps);
+        float undo;
+        const float mul = ka_q_scale(max(max(tops.x, tops.y), max(tops.z, tops.w)), &undo);
+        sc[k] = fmaxf(a.scale_log2 * undo, 1e-37f);  // never 0: 0 x -inf
+        const float f = a.negate ? -mul : mul;
         uint32_t* q32 = reinterpret_cast<uint32_t*>(qfrag);
 #pragma unroll
-        for (int s = 0; s < 2 * KW; ++s)
-          if (s % kKaWarps == warp) {
-            q32[(s * 32 + lane) * 4 + k] = h[2 * s];
-            q32[(s * 32 + lane) * 4 + 2 + k] = h[2 * s + 1];
-          }
-        rowpos[k] = it.x.pos + max(i, 0);
+        for (int i = 0; i < QW; ++i)  // steps QW / 2 x warp + i / 2
+          q32[((warp * (QW / 2) + i / 2) * 32 + lane) * 4 + (i & 1) * 2 + k] = ka_h2(bf_lo(qv[k][i]) * f, bf_hi(qv[k][i]) * f);
       }
       ka_sync();
       float o[NV][4];
@@ -602,13 +634,12 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
         return reinterpret_cast<float4*>(join + (w * kKaRows + r) * D + (column ^ (r & 1)) * NV +
                                          4 * (piece ^ (D == 128 ? column >> 1 : column >> 2)));
       };
-      ka_sync();  // q's operands are no longer read
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int r = g + 8 * k;
         if (t == 0) {
-          join_m[warp * kKaRows + r] = m[k];
-          join_l[warp * kKaRows + r] = l[2 * k];
+          join_m[r * kKaWarps + warp] = m[k];
+          join_l[r * kKaWarps + warp] = l[2 * k];
         }
 #pragma unroll
         for (int col = 0; col < 2; ++col)
@@ -628,28 +659,33 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
       }
       // a CTA's range holds one item's end and another's beginning at most: two records per CTA
       auto slot_of = [&](int p) { return 2 * (first + p) + (ka_range(it, first + p) < u0 ? 1 : 0); };
-      auto out_at = [&](int r, int d) {
-        return a.out + ((int64_t)it.b * a.T + row_token[r]) * a.out_stride + row_head[r] * D + d;
+      auto finish = [&](int r, int d, float4 v, float sum) {
+        const int row = it.tile * kKaRows + r, i = ka_div_g(a, row);
+        if (row >= a.G * a.T) return;
+        const bool on = i < used;
+        ka_store(a.out + ((int64_t)it.b * a.T + i) * a.out_stride + (int64_t)(it.h * a.G + row - i * a.G) * D + d,
+                 on ? v : make_float4(0.f, 0.f, 0.f, 0.f), on ? sum : 0.f);
       };
       const int my_part = blockIdx.x - first;
       float* rec = whole ? nullptr : a.parts + (size_t)slot_of(my_part) * S::kRecord;
-#pragma unroll 1
-      for (int e = tid; e < kKaRows * D / 4; e += kKaWarps * 32) {
-        const int r = e / (D / 4), d = e % (D / 4) * 4;
-        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kKaRows * D / 4 / (kKaWarps * 32); ++k) {
+        const int e = tid + k * kKaWarps * 32, r = e / (D / 4), d = e % (D / 4) * 4;
+        const float4 mw = *reinterpret_cast<const float4*>(join_m + r * kKaWarps);
+        const float4 lw = *reinterpret_cast<const float4*>(join_l + r * kKaWarps);
+        const float top = fmaxf(fmaxf(mw.x, mw.y), fmaxf(mw.z, mw.w));
+        const float ms[4] = {mw.x, mw.y, mw.z, mw.w}, ls[4] = {lw.x, lw.y, lw.z, lw.w};
+        float sum = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < kKaWarps; ++w) top = fmaxf(top, join_m[w * kKaRows + r]);
-#pragma unroll
         for (int w = 0; w < kKaWarps; ++w) {
-          const float mw = join_m[w * kKaRows + r], f = mw == -INFINITY ? 0.f : ka_exp2(mw - top);
+          const float f = ms[w] == -INFINITY ? 0.f : ka_exp2(ms[w] - top);
           const float4 x = *at(w, r, d / NV, d % NV / 4);
-          sum += join_l[w * kKaRows + r] * f;
+          sum += ls[w] * f;
           v = make_float4(v.x + x.x * f, v.y + x.y * f, v.z + x.z * f, v.w + x.w * f);
         }
         if (whole) {
-          const bool on = row_token[r] < used;
-          if (row_token[r] >= 0) ka_store(out_at(r, d), on ? v : make_float4(0.f, 0.f, 0.f, 0.f), on ? sum : 0.f);
+          finish(r, d, v, sum);
         } else {
           *reinterpret_cast<float4*>(rec + r * D + d) = v;
           if (d == 0) {
@@ -666,11 +702,14 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
         const int members = min(kKaFan, count - lead);
         const bool final = count <= kKaFan;
         if (members > 1) {
-          __threadfence();
           ka_sync();
           if (tid == 0) {
+            // the barrier orders every thread's stores before this release, and the others' loads after
+            // this acquire by the next one
             uint32_t* ctr = a.arrived + level * 2 * gridDim.x + slot_of(lead * span);
-            const bool last = atomicAdd(ctr, 1u) == (uint32_t)members - 1;
+            uint32_t before;
+            asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(ctr) : "memory");
+            const bool last = before == (uint32_t)members - 1;
             if (last) *ctr = 0;
             flags[1] = last;
           }
@@ -678,7 +717,17 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
             recs[tid - 32] = a.parts + (size_t)slot_of((lead + min(tid - 32, members - 1)) * span) * S::kRecord;
           ka_sync();
           if (!flags[1]) break;
-          __threadfence();
+          // this thread's 16-byte pieces, four parts of each at a time: 16 loads in flight
+          constexpr int kMine = kKaRows * D / 4 / (kKaWarps * 32);
+          float4 v[kMine][4];
+          auto load = [&](int q0) {
+#pragma unroll
+            for (int k = 0; k < kMine; ++k)
+#pragma unroll
+              for (int p = 0; p < 4; ++p)
+                v[k][p] = __ldcg(reinterpret_cast<const float4*>(recs[q0 + p]) + tid + k * kKaWarps * 32);
+          };
+          load(0);
           // thread (part group, row): maxima and sums of two parts
           float* wgt = join;                    // [16 parts][16 rows]
           float* sums = join + kKaFan * kKaRows;
@@ -712,19 +761,12 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
           }
           ka_sync();
           float* dst = recs[0];
-          // this thread's 16-byte pieces, four parts of each at a time: 16 loads in flight
-          constexpr int kMine = kKaRows * D / 4 / (kKaWarps * 32);
           float4 acc[kMine];
 #pragma unroll
           for (int k = 0; k < kMine; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
           for (int q0 = 0; q0 < members; q0 += 4) {
-            float4 v[kMine][4];
-#pragma unroll
-            for (int k = 0; k < kMine; ++k)
-#pragma unroll
-              for (int p = 0; p < 4; ++p)
-                v[k][p] = __ldcg(reinterpret_cast<const float4*>(recs[q0 + p]) + tid + k * kKaWarps * 32);
+            if (q0) load(q0);
 #pragma unroll
             for (int p = 0; p < 4; ++p)
               if (q0 + p < members)
@@ -739,8 +781,7 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
           for (int k = 0; k < kMine; ++k) {
             const int e = tid + k * kKaWarps * 32, r = e / (D / 4), d = e % (D / 4) * 4;
             if (final) {
-              const bool on = row_token[r] < used;
-              if (row_token[r] >= 0) ka_store(out_at(r, d), on ? acc[k] : make_float4(0.f, 0.f, 0.f, 0.f), on ? join_l[r] : 0.f);
+              finish(r, d, acc[k], join_l[r]);
             } else {
               *reinterpret_cast<float4*>(dst + r * D + d) = acc[k];
               if (d == 0) {
@@ -755,10 +796,8 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
         count = (count + kKaFan - 1) / kKaFan;
         span *= kKaFan;
       }
-      if (a.listed && it.w + it.c1 - it.c0 >= it.w1) break;  // the CTA's last
-      ka_sync();
-      if (tid == 0) ka_next(a, cum, &it);
-      ka_sync();
+      ka_sync();  // (the joining buffers are free, the place is read)
+      if (lane == 0) tc_arrive(&ended[item & 1]);
   }
 
   // rows of items without a chunk
@@ -850,7 +889,7 @@ extern "C" int jsx_kv4_attn(const void* q, int64_t q_stride, const void* pool, i
   a.pt_log = page_tokens == 16 ? 4 : page_tokens == 32 ? 5 : page_tokens == 64 ? 6 : 7;
   a.window = window < (1 << 30) ? window : 1 << 30;  // (positions are below 2^30)
   a.sinks = sinks;
-  a.negate = scale < 0.f ? 0x80000000u : 0u;
+  a.negate = scale < 0.f;
   a.scale_log2 = fabsf(scale) * 1.4426950408889634f;
   const int64_t items = (int64_t)B * nkv * a.tiles;
   const int64_t chunks = items * (((int64_t)table_slots * page_tokens + kKaChunk - 1) / kKaChunk);
