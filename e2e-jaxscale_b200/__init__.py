@@ -10,7 +10,9 @@ from . import weights  # noqa: F401
 from .config import ModelConfig  # noqa: F401
 from .glm4 import DecodeGraph, DecodeState, GLM4ForCausalLM, PrefillState  # noqa: F401
 from .flash import GLM4FlashForCausalLM  # noqa: F401
+from .layers.paged_cache import PagedKV4Cache  # noqa: F401
 from .mesh import Comm, Mesh, create_mesh  # noqa: F401
 from .runner import JittedModel, greedy_generate, sample_generate  # noqa: F401
+from .speculative import speculative_generate  # noqa: F401
 
 __version__ = "0.1.0"
