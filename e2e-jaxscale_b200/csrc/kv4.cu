@@ -10,9 +10,11 @@
 // bf16 bit patterns, where NaN is above infinity: a group with a NaN gets a NaN
 // scale and reads back as NaN; infinities saturate at 6 x 448.
 //
-// Both kernels are bound by memory: 32 bytes of bf16 per 9 bytes of page.  One
-// thread handles one group: two 16-byte accesses on the bf16 side, 8 bytes of
-// codes and one scale byte on the page side; the threads of a row are adjacent.
+// Both kernels move 32 bytes of bf16 per 9 bytes of page.  One thread handles a group
+// of a K row and the same of its V row: two 16-byte accesses each on the bf16 side, 8
+// bytes of codes and one scale byte on the page side; the threads of a row are adjacent.
+// (8 values a thread would make every access whole, but doubles the index arithmetic:
+// 30 against 23 us for 32 x 1024 rows of 2 heads there and back.)
 #include "common.cuh"
 #include "kv4.cuh"
 #include "launch.cuh"
@@ -30,96 +32,111 @@ struct Kv4RowArgs {
   const int32_t* table;
   const int32_t* positions;
   const int32_t* n_tokens;
-  int num_pages, slots, T, nkv, pt;
-  int64_t units;  // B * T * nkv * 2 * (D / 16)
+  int num_pages, slots, nkv, pt, pt_log;
+  uint32_t units;  // of a sequence: T * nkv * (D / 16)
 };
 
-// Where unit u lies: its 16 values in the row, and its block, token slot and group in the pool.
+// Where unit u of sequence b, 16 values of a K row and the same of its V row, lies: in the
+// rows (row), and in its block of the pool.  (32-bit indexes inside a sequence, and K and V
+// together: finding the place is what these kernels spend most instructions on.)
 struct Kv4Unit {
-  bf16* row;
-  uint8_t* codes;
-  uint8_t* scale;
-  bool inside;  // the row exists (token used, position inside the static cache)
-  bool paged;   // ... and has a page
+  int64_t row;     // elements from k and from v
+  uint8_t* codes;  // of K; V's are kv4_off_v further
+  uint8_t* scale;  // of K; V's pt * D / 16 further
+  bool inside;     // the row exists (token used, position inside the static cache)
+  bool paged;      // ... and has a page
 };
 
 template <int D>
-__device__ __forceinline__ Kv4Unit kv4_unit(const Kv4RowArgs& a, int64_t u) {
+__device__ __forceinline__ Kv4Unit kv4_unit(const Kv4RowArgs& a, int b, uint32_t u, int first, int used) {
   constexpr int NG = D / kKv4Group;
   const int g = (int)(u % NG);
-  const int64_t r = u / NG;
-  const int which = (int)(r & 1);
-  const int64_t mh = r >> 1;
-  const int h = (int)(mh % a.nkv);
-  const int64_t m = mh / a.nkv;
-  const int b = (int)(m / a.T), i = (int)(m % a.T);
-  const int pos = a.positions[b] + i;
+  const uint32_t mh = u / NG;
+  const int i = (int)(mh / (uint32_t)a.nkv), h = (int)(mh - (uint32_t)i * a.nkv);
+  const int pos = first + i;
   Kv4Unit x;
-  x.inside = (!a.n_tokens || i < a.n_tokens[b]) && pos >= 0 && (a.cache_rows == 0 || pos < a.cache_rows);
-  x.row = (which ? a.v : a.k) + b * a.seq_stride + (int64_t)(a.cache_rows ? pos : i) * a.token_stride +
-          h * a.head_stride + g * kKv4Group;
-  const int slot = pos / a.pt;
+  x.inside = u < a.units && i < used && pos >= 0 && (a.cache_rows == 0 || pos < a.cache_rows);
+  x.row = b * a.seq_stride + (int64_t)(a.cache_rows ? pos : i) * a.token_stride + h * a.head_stride + g * kKv4Group;
+  const int slot = pos >> a.pt_log;
   int page = -1;
   if (x.inside && slot < a.slots) page = a.table[(int64_t)b * a.slots + slot];
   x.paged = page >= 0 && page < a.num_pages;
-  const int t = pos - slot * a.pt;
+  const int t = pos & (a.pt - 1);
   uint8_t* block = a.pool + ((int64_t)page * a.nkv + h) * kv4_block_bytes(a.pt, D);
-  x.codes = block + (which ? kv4_off_v(a.pt, D) : 0) + t * (D / 2) + g * 8;
-  x.scale = block + (which ? kv4_off_vs(a.pt, D) : kv4_off_ks(a.pt, D)) + t * NG + g;
+  x.codes = block + t * (D / 2) + g * 8;
+  x.scale = block + kv4_off_ks(a.pt, D) + t * NG + g;
   return x;
 }
 
 template <int D>
 __global__ void __launch_bounds__(kKv4Threads) k_kv4_append(Kv4RowArgs a) {
   pdl_wait();
-  const int64_t step = (int64_t)gridDim.x * kKv4Threads;
-  for (int64_t u = (int64_t)blockIdx.x * kKv4Threads + threadIdx.x; u < a.units; u += step) {
-    const Kv4Unit x = kv4_unit<D>(a, u);
-    if (!x.paged) continue;
-    const uint4 p0 = *reinterpret_cast<const uint4*>(x.row), p1 = *reinterpret_cast<const uint4*>(x.row + 8);
-    const uint32_t w[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
-    uint32_t mx = 0;
+  const int b = blockIdx.y, first = a.positions[b], used = a.n_tokens ? a.n_tokens[b] : INT32_MAX;
+  for (uint32_t u = blockIdx.x * kKv4Threads + threadIdx.x; u < a.units; u += gridDim.x * kKv4Threads) {
+    const Kv4Unit x = kv4_unit<D>(a, b, u, first, used);
+    if (!x.inside) continue;
+    uint4 p[2][2];  // in flight together with the page number
 #pragma unroll
-    for (int i = 0; i < 8; ++i) mx = __vmaxu2(mx, w[i] & 0x7fff7fffu);
-    const float top = __uint_as_float(max(mx & 0xffffu, mx >> 16) << 16);
-    const uint32_t sc = f32_to_e4m3(__fdiv_rn(top, 6.f));
-    const float s = __half2float(__ushort_as_half((unsigned short)(e4m3x2_to_h2(sc) & 0xffffu)));
-    const float inv = s == 0.f ? 0.f : __frcp_rn(s);
-    float q[2][8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      q[i >> 2][2 * (i & 3)] = __fmaf_rn(bf_lo(w[i]), inv, 1536.f) - 1536.f;
-      q[i >> 2][2 * (i & 3) + 1] = __fmaf_rn(bf_hi(w[i]), inv, 1536.f) - 1536.f;
+    for (int k = 0; k < 2; ++k) {
+      const bf16* row = (k ? a.v : a.k) + x.row;
+      p[k][0] = *reinterpret_cast<const uint4*>(row);
+      p[k][1] = *reinterpret_cast<const uint4*>(row + 8);
     }
-    *reinterpret_cast<uint2*>(x.codes) = make_uint2(f32x8_to_e2m1(q[0]), f32x8_to_e2m1(q[1]));
-    *x.scale = (uint8_t)sc;
+    if (!x.paged) continue;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t w[8] = {p[k][0].x, p[k][0].y, p[k][0].z, p[k][0].w, p[k][1].x, p[k][1].y, p[k][1].z, p[k][1].w};
+      uint32_t mx = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = __vmaxu2(mx, w[i] & 0x7fff7fffu);
+      const float top = __uint_as_float(max(mx & 0xffffu, mx >> 16) << 16);
+      const uint32_t sc = f32_to_e4m3(__fdiv_rn(top, 6.f));
+      const float s = __half2float(__ushort_as_half((unsigned short)(e4m3x2_to_h2(sc) & 0xffffu)));
+      const float inv = s == 0.f ? 0.f : __frcp_rn(s);
+      float q[2][8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        q[i >> 2][2 * (i & 3)] = __fmaf_rn(bf_lo(w[i]), inv, 1536.f) - 1536.f;
+        q[i >> 2][2 * (i & 3) + 1] = __fmaf_rn(bf_hi(w[i]), inv, 1536.f) - 1536.f;
+      }
+      *reinterpret_cast<uint2*>(x.codes + k * kv4_off_v(a.pt, D)) = make_uint2(f32x8_to_e2m1(q[0]), f32x8_to_e2m1(q[1]));
+      x.scale[k * a.pt * (D / kKv4Group)] = (uint8_t)sc;
+    }
   }
 }
 
 template <int D>
 __global__ void __launch_bounds__(kKv4Threads) k_kv4_read(Kv4RowArgs a) {
   pdl_wait();
-  const int64_t step = (int64_t)gridDim.x * kKv4Threads;
-  for (int64_t u = (int64_t)blockIdx.x * kKv4Threads + threadIdx.x; u < a.units; u += step) {
-    const Kv4Unit x = kv4_unit<D>(a, u);
+  const int b = blockIdx.y, first = a.positions[b], used = a.n_tokens ? a.n_tokens[b] : INT32_MAX;
+  for (uint32_t u = blockIdx.x * kKv4Threads + threadIdx.x; u < a.units; u += gridDim.x * kKv4Threads) {
+    const Kv4Unit x = kv4_unit<D>(a, b, u, first, used);
     if (!x.inside) continue;
-    uint32_t o[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+    uint2 c[2] = {};
+    uint32_t sc[2] = {};
     if (x.paged) {
-      const uint2 c = *reinterpret_cast<const uint2*>(x.codes);
-      const uint32_t sc = *x.scale;
-      const uint32_t s2 = e4m3x2_to_h2(sc | (sc << 8));
-      uint32_t h[8];
-      e2m1x8_to_h2(c.x, reinterpret_cast<uint32_t(&)[4]>(h[0]));
-      e2m1x8_to_h2(c.y, reinterpret_cast<uint32_t(&)[4]>(h[4]));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        c[k] = *reinterpret_cast<const uint2*>(x.codes + k * kv4_off_v(a.pt, D));
+        sc[k] = x.scale[k * a.pt * (D / kKv4Group)];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t s2 = e4m3x2_to_h2(sc[k] | (sc[k] << 8));
+      uint32_t h[8], o[8];
+      e2m1x8_to_h2(c[k].x, reinterpret_cast<uint32_t(&)[4]>(h[0]));
+      e2m1x8_to_h2(c[k].y, reinterpret_cast<uint32_t(&)[4]>(h[4]));
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t y = hmul2_u(h[i], s2);
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&y));
         o[i] = pack2(f.x, f.y);
       }
+      bf16* row = (k ? a.v : a.k) + x.row;
+      *reinterpret_cast<uint4*>(row) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4*>(row + 8) = make_uint4(o[4], o[5], o[6], o[7]);
     }
-    *reinterpret_cast<uint4*>(x.row) = make_uint4(o[0], o[1], o[2], o[3]);
-    *reinterpret_cast<uint4*>(x.row + 8) = make_uint4(o[4], o[5], o[6], o[7]);
   }
 }
 
@@ -129,7 +146,8 @@ static int kv4_rows(bool append, const void* k, const void* v, int64_t seq_strid
                     int head_dim, int page_tokens, void* stream) {
   JSX_REQUIRE(k && v && positions, "null pointer argument");
   JSX_KV4_REQUIRE(pool, num_pages, table, table_slots, nkv, head_dim, page_tokens);
-  JSX_REQUIRE(B >= 1 && T >= 1 && cache_rows >= 0, "B=%d T=%d cache_rows=%d", B, T, cache_rows);
+  JSX_REQUIRE(B >= 1 && B <= 65535 && T >= 1 && cache_rows >= 0, "B=%d (1..65535) T=%d cache_rows=%d", B, T, cache_rows);
+  JSX_REQUIRE((int64_t)T * nkv * (head_dim / kKv4Group) < (1ll << 30), "%d tokens of %d kv heads per sequence", T, nkv);
   JSX_REQUIRE(aligned16(k) && aligned16(v) && seq_stride % 8 == 0 && token_stride % 8 == 0 && head_stride % 8 == 0,
               "rows must be 16-byte aligned");
   JSX_REQUIRE(seq_stride >= 0 && token_stride >= 0 && head_stride >= 0, "negative stride");
@@ -146,12 +164,12 @@ static int kv4_rows(bool append, const void* k, const void* v, int64_t seq_strid
   a.n_tokens = n_tokens;
   a.num_pages = num_pages;
   a.slots = table_slots;
-  a.T = T;
   a.nkv = nkv;
   a.pt = page_tokens;
-  a.units = (int64_t)B * T * nkv * 2 * (head_dim / kKv4Group);
-  const int64_t blocks = (a.units + kKv4Threads - 1) / kKv4Threads;
-  const dim3 grid((unsigned)(blocks < 8ll * sm_count() ? blocks : 8ll * sm_count()));
+  a.pt_log = page_tokens == 16 ? 4 : page_tokens == 32 ? 5 : page_tokens == 64 ? 6 : 7;
+  a.units = (uint32_t)T * nkv * (head_dim / kKv4Group);
+  const uint32_t blocks = (a.units + kKv4Threads - 1) / kKv4Threads, most = (16u * sm_count() + B - 1) / B;
+  const dim3 grid(blocks < most ? blocks : most, B);
   auto kern = append ? (head_dim == 128 ? k_kv4_append<128> : k_kv4_append<64>)
                      : (head_dim == 128 ? k_kv4_read<128> : k_kv4_read<64>);
   JSX_CUDA(launch_kernel(kern, grid, dim3(kKv4Threads), 0, (cudaStream_t)stream, a));

@@ -590,7 +590,7 @@ def kv4_attn(q, pool, table, positions, head_dim, workspace, scale=None, tokens_
     if not q.is_cuda or q.dtype != BF16:
         raise TypeError("q must be a bf16 CUDA tensor")
     if out is None:
-        out = torch.empty(q.shape, dtype=BF16, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != BF16 or out.stride(1) != 1 or not out.is_cuda:
         raise ValueError("out must be a bf16 CUDA tensor of q's shape")
     call("jsx_kv4_attn", q.data_ptr(), q.stride(0), pool.data_ptr(), P_, table.data_ptr(), slots, positions.data_ptr(),
@@ -651,7 +651,7 @@ def pages_resize(table, held, refs, keep, need, pool, page_tokens, workspace, mi
     if keep.numel() != S or need.numel() != S:
         raise ValueError(f"keep and need must have one entry per sequence ({S})")
     layers, page_bytes = _pages_pool(pool, P_)
-    missing = torch.empty(1, dtype=I32, device=table.device) if missing is None else _need(missing, "missing", I32)
+    missing = held.new_empty(1) if missing is None else _need(missing, "missing", I32)
     call("jsx_pages_resize", table.data_ptr(), held.data_ptr(), refs.data_ptr(), keep.data_ptr(), need.data_ptr(),
          pool.data_ptr(), layers, page_bytes, S, slots, P_, page_tokens, missing.data_ptr(), workspace.data_ptr(),
          workspace.numel(), _stream())
@@ -705,8 +705,8 @@ def verify_drafts(logits, draft_ids, uniforms, workspace, draft_probs=None, n_dr
         raise ValueError("draft_ids [B, T], uniforms [B, T + 1], draft_probs [B, T, V] and n_draft [B] must match logits")
     dev = logits.device
     accepted = torch.empty(B, dtype=I32, device=dev) if accepted is None else _need(accepted, "accepted", I32)
-    tokens = torch.empty((B, T + 1), dtype=I32, device=dev) if tokens is None else _need(tokens, "tokens", I32)
-    accept_prob = (torch.empty((B, T), dtype=torch.float32, device=dev) if accept_prob is None
+    tokens = draft_ids.new_empty((B, T + 1)) if tokens is None else _need(tokens, "tokens", I32)
+    accept_prob = (torch.empty_strided((B, T), (T, 1), dtype=torch.float32, device=dev) if accept_prob is None
                    else _need(accept_prob, "accept_prob", torch.float32))
     if accepted.numel() != B or tokens.numel() != B * (T + 1) or accept_prob.numel() != B * T:
         raise ValueError("accepted [B], tokens [B, T + 1] and accept_prob [B, T] must match logits")
