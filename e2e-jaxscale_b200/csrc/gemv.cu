@@ -782,6 +782,7 @@ int read_clear_step_error(uint32_t* out);  // decode_step.cu
 int read_clear_tc_error(uint32_t* out);    // tc_gemm.cu
 int read_clear_wide_error(uint32_t* out);  // tc_wide.cu
 int read_clear_kv4_error(uint32_t* out);   // kv4_attn.cu
+int read_clear_kv4_wide_error(uint32_t* out);  // kv4_attn_wide.cu
 }
 
 extern "C" int jsx_device_error(int* status) {
@@ -804,6 +805,9 @@ extern "C" int jsx_device_error(int* status) {
   uint32_t x = 0;
   st = jsx::read_clear_kv4_error(&x);
   if (st != JSX_OK) return st;
-  *status = (v | w | t | u | x) ? JSX_ETIMEDOUT : JSX_OK;
+  uint32_t y = 0;
+  st = jsx::read_clear_kv4_wide_error(&y);
+  if (st != JSX_OK) return st;
+  *status = (v | w | t | u | x | y) ? JSX_ETIMEDOUT : JSX_OK;
   return JSX_OK;
 }

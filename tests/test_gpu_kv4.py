@@ -248,6 +248,40 @@ def test_attention_nan_reaches_only_its_rows(jsx, cuda):
     assert bad[0, 1, :, :16].all() and not bad[0, 0].any() and not bad[1].any() and not bad[0, 1, :, 16:].any()
 
 
+@pytest.mark.parametrize("T,nq,hd", [(2, 8, 128), (5, 16, 128), (4, 4, 64)])
+def test_attention_nan_that_only_some_tokens_see(jsx, cuda, T, nq, hd):
+    """V rows with a NaN inside one token's window and outside another's, K rows too: the tokens that
+    do not see them are as without it, the others NaN in that row's 16 dimensions (V) or all (K)."""
+    rng = np.random.default_rng(T)
+    L, window, first = 300, 64, 250
+    t, pages = make_table(rng, [L], 32)
+    k, v = rows(rng, 1, L, 1, hd), rows(rng, 1, L, 1, hd)
+    q = rows(rng, T, nq * hd)
+    ws = jsx.kernels.kv4_attn_workspace(1, T, nq, 1, hd, q.device)
+
+    def run(kk, vv):
+        pool = make_pool(jsx, pages, 1, hd, 32)
+        jsx.kernels.kv4_append(kk, vv, pool, dev(t), dev([0]), tokens_per_seq=L)
+        o = jsx.kernels.kv4_attn(q, pool, dev(t), dev([first]), hd, ws, tokens_per_seq=T, window=window)
+        return o.view(T, nq, hd)
+
+    clean = run(k, v)
+    oldest = first - window + 1          # token 0's oldest row: no other token sees it
+    newest = first + T - 1               # the last token's own row
+    vv = v.clone()
+    vv[0, oldest, 0, 17] = float("nan")
+    vv[0, newest, 0, 40] = float("nan")
+    o = run(k, vv)
+    want = torch.zeros(T, nq, hd, dtype=torch.bool, device="cuda")
+    want[0, :, 16:32] = True
+    want[T - 1, :, 32:48] = True
+    assert torch.equal(torch.isnan(o), want) and torch.equal(o[~want], clean[~want])
+    kk = k.clone()
+    kk[0, newest, 0, 3] = float("nan")
+    o = run(kk, v)
+    assert torch.isnan(o[T - 1]).all() and torch.equal(o[:T - 1], clean[:T - 1])
+
+
 def test_attention_missing_pages_and_short_tables(jsx, cuda):
     def holes(t):
         t = t.copy()
