@@ -586,8 +586,28 @@ __global__ void __launch_bounds__(kKaThreads, kKaPerSm) k_kv4_attn(const __grid_
 // kv4_attn_wide.cu: items of 128 query rows
 size_t kv4_wide_workspace(int B, int T, int nq, int nkv);
 int kv4_wide_launch(KaArgs a, void* workspace, cudaStream_t s);
-// From 33 query rows per kv head on (three 16-row items or more would convert every cache row again).
-static bool ka_wide(int T, int nq, int nkv, int head_dim) { return head_dim == 128 && (int64_t)nq / nkv * T > 32; }
+
+// Chunks per item of the rows that a call can see, by the table and the window (the lengths
+// are on the device).
+static int64_t ka_chunks(int64_t table_rows, int T, int window, int sinks) {
+  const int64_t seen = window > 0 ? (int64_t)window + T + sinks + 2 * kKaChunk : table_rows;
+  return ((seen < table_rows ? seen : table_rows) + kKaChunk - 1) / kKaChunk;
+}
+// Which kernel: fitted to both, the 16-row one takes 10 us + 3.5 ns and the 128-row one
+// 20 us + 10.7 ns per chunk of an item, so the latter begins to pay where it saves the 16-row
+// kernel 2048 chunks beyond three times its own.  Where each sequence has a count of tokens
+// of its own, half of T are taken to be used.  head_dim 128, 16-row / 128-row kernel, us:
+//   32 heads on 2, 16 sequences of up to 8192 rows: T 2: 27 / 40, 4: 40 / 41, 5: 48 / 41,
+//     8: 70 / 45, 16: 130 / 64, 64: 490 / 198;  5 with counts of 0 to 5: 36 / 42
+//   8 heads on 1, 64 sequences of up to 4000 rows: T 5: 36 / 39, 9: 51 / 42, 16: 76 / 47
+//   32 heads on 2, one sequence of 4000 rows: T 8: 17 / 23, 33: 29 / 34, 64: 44 / 34
+// Up to 48 query rows per kv head it never does.
+static bool ka_wide_ever(int T, int nq, int nkv, int head_dim) { return head_dim == 128 && (int64_t)(nq / nkv) * T > 3 * kKaRows; }
+static bool ka_wide(int B, int T, int nq, int nkv, int head_dim, bool counts, int64_t chunks) {
+  if (!ka_wide_ever(T, nq, nkv, head_dim)) return false;
+  const int64_t rows = (int64_t)(nq / nkv) * (counts ? (T + 1) / 2 : T), lists = (int64_t)B * nkv * chunks;
+  return lists * ((rows + kKaRows - 1) / kKaRows) - 3 * lists * ((rows + 127) / 128) >= 2048;
+}
 
 // CTAs of a launch: kKaPerSm per SM, or as many as there are chunks (items) at most.
 static int ka_grid_max() { return kKaPerSm * sm_count(); }
@@ -614,11 +634,9 @@ using namespace jsx;
 extern "C" int jsx_kv4_attn_workspace_size(int B, int T, int nq, int nkv, int head_dim, size_t* bytes) {
   JSX_REQUIRE(bytes && B >= 1 && T >= 1 && nq >= 1 && nkv >= 1 && nq % nkv == 0 && (head_dim == 64 || head_dim == 128),
               "bad arguments");
-  if (ka_wide(T, nq, nkv, head_dim)) {
-    *bytes = kv4_wide_workspace(B, T, nq, nkv);
-    return JSX_OK;
-  }
-  *bytes = ka_arrived_bytes() + 2 * (size_t)ka_grid_max() * ka_record_bytes(head_dim);
+  const size_t records = 2 * (size_t)ka_grid_max() * ka_record_bytes(head_dim);
+  const size_t wide = ka_wide_ever(T, nq, nkv, head_dim) ? kv4_wide_workspace(B, T, nq, nkv) : 0;
+  *bytes = ka_arrived_bytes() + (wide > records ? wide : records);
   return JSX_OK;
 }
 
@@ -669,7 +687,8 @@ extern "C" int jsx_kv4_attn(const void* q, int64_t q_stride, const void* pool, i
   a.sinks = sinks;
   a.negate = scale < 0.f;
   a.scale_log2 = fabsf(scale) * 1.4426950408889634f;
-  if (ka_wide(T, nq, nkv, head_dim)) return kv4_wide_launch(a, workspace, (cudaStream_t)stream);
+  if (ka_wide(B, T, nq, nkv, head_dim, n_tokens != nullptr, ka_chunks((int64_t)table_slots * page_tokens, T, a.window, sinks)))
+    return kv4_wide_launch(a, a.parts, (cudaStream_t)stream);
   const int64_t items = (int64_t)B * nkv * a.tiles;
   const int64_t chunks = items * (((int64_t)table_slots * page_tokens + kKaChunk - 1) / kKaChunk);
   a.listed = (int64_t)B * a.tiles <= kKaListMax && chunks < (1 << 30);

@@ -2,26 +2,40 @@
 // per sequence): items of 128 rows on the tcgen05 tensor cores, head_dim 128.
 //
 // The kernel of 16-row items (kv4_attn.cu) converts every cache row again for each 16 query
-// rows, and its MMA, conversions and multiplications share the issue slots; here a cache row is converted
-// once for 128 query rows and both products are issued by one thread.  Per 64 cache rows:
-//   warps 6..13  codes -> f16 operands in shared memory, 128-byte swizzled: K [64][128] as it is,
-//                V transposed to [128][64] (the nibbles of two rows interleaved before the
-//                conversion give a pair along the summed axis);
-//   warp 5       S = Q K^T (M 128, N 64, K 128) into one of two TMEM accumulators, then
-//                O += P V (M 128, N 128, K 64) once P is there;
-//   warps 0..3   a thread per query row: tcgen05.ld of its 64 scores, mask, running reference,
-//                weights as f16 into P; O stays in TMEM and is rescaled there on the rare
-//                occasions that a row's reference moves;
-//   warp 4       places and pages (cp.async.bulk), running ahead.
-// S of step n + 1 is issued before P of step n is waited for, so conversions, products and
-// weights of neighbouring steps overlap.  A stored value is exact in f16, q is scaled by a
-// power of two per row, P has 11 bits: the same roundings as the 16-row kernel's.
+// rows, and its MMA, conversions and multiplications share the issue slots; here a cache row
+// is converted once for 128 query rows and each product is issued by one thread.  Per step of
+// 64 cache rows:
+//   warps 10..17 codes -> f16 operands in shared memory, 128-byte swizzled, three steps ahead:
+//                K [64][128] as it is (four warps), V transposed to [128][64] (four; the nibbles
+//                of two rows interleaved before the conversion give a pair along the summed
+//                axis).  Which 16 bytes of a row a lane reads moves with the lane: rows are 64
+//                bytes apart, read straight they met in two bank groups (365 of 741 wavefronts
+//                a step were conflicts, now 69 of 424);
+//   warp 9       S = Q K^T (M 128, N 64, K 128) into one of four TMEM accumulators;
+//   warp 18      O += P V (M 128, N 128, K 64) once P is there.  Two warps, and elect.sync rather
+//                than a lane's branch, because issuing the twelve products is itself long
+//                (64 tokens x 16 sequences of 8191: 235 -> 205 us by elect, 198 by two warps);
+//   warps 0..3   a thread per query row, for even steps: tcgen05.ld of its 64 scores, mask,
+//                running reference, weights as f16 into P; O stays in TMEM and is rescaled there
+//                on the rare occasions that a row's reference moves;
+//   warps 4..7   the same for odd steps, with a reference and an O of their own; the two meet at
+//                an item's end (with one group of four every scheduler waited for one warp);
+//   warp 8       places and pages (cp.async.bulk), running ahead.
+// A stored value is exact in f16, q is scaled by a power of two per row, P has 11 bits: the
+// same roundings as the 16-row kernel's.
+//
+// Bound: the softmax warps, two per scheduler, which are busy all the time: 64 exponentials,
+// their conversions and sums take 1300 cycles of a step's 2700 and share the issue slots (55%
+// taken) with the conversions; an item's first rows and its end cost about 6 us a CTA, the
+// joining launch 7.  32 heads on 2, 16 sequences of up to 8191 rows: 41 us for 5 tokens, 64 for
+// 16, 198 for 64 (the 16-row kernel: 48, 130, 490), which is 0.45 PFLOP/s at 64.
 //
 // NaN: a row's NaN scale enters V as 0 (it would reach every query row through weights of
 // 0) and is noted; the query rows that see it get their NaN when they are written.
 //
 // Items that several CTAs share leave (output, maximum, sum) records, which a second launch
-// joins, 16 rows per CTA, in part order.
+// joins, 16 rows per CTA, in part order: a record is 64 KB, and more CTAs than there are
+// items read them.
 #include "kv4_attn.cuh"
 #include "launch.cuh"
 
@@ -31,18 +45,19 @@ constexpr int kKwRows = 128;
 constexpr int kKwStep = 64;  // cache rows per product
 constexpr int kKwD = 128;
 constexpr int kKwStages = 3;
-constexpr int kKwThreads = 14 * 32;
-constexpr int kKwCopyWarp = 4, kKwMmaWarp = 5, kKwKWarp = 6, kKwVWarp = 10;
+constexpr int kKwBufs = 3;  // steps of operands ahead
+constexpr int kKwThreads = 19 * 32;
+constexpr int kKwCopyWarp = 8, kKwMmaWarp = 9, kKwKWarp = 10, kKwVWarp = 14, kKwPvWarp = 18;
 constexpr int kKwStage = kv4_block_bytes(kKaChunk, kKwD);
 constexpr int kKwQBytes = kKwRows * kKwD * 2;       // two blocks of [128 rows][64]
 constexpr int kKwKBytes = kKwStep * kKwD * 2;       // two blocks of [64 rows][64]
 constexpr int kKwVBytes = kKwD * kKwStep * 2;       // [128 dimensions][64 rows]
 constexpr int kKwPBytes = kKwRows * kKwStep * 2;    // [128 query rows][64 rows]
-constexpr int kKwOffK = kKwQBytes, kKwOffV = kKwOffK + 2 * kKwKBytes, kKwOffP = kKwOffV + 2 * kKwVBytes;
+constexpr int kKwOffK = kKwQBytes, kKwOffV = kKwOffK + kKwBufs * kKwKBytes, kKwOffP = kKwOffV + kKwBufs * kKwVBytes;
 constexpr int kKwOffRing = kKwOffP + 2 * kKwPBytes;
 constexpr int kKwSmem = kKwOffRing + kKwStages * kKwStage + 1024 /* align */;
-constexpr uint32_t kKwTmemCols = 256, kKwTmemO = 128;  // S 0..63, 64..127, O 128..255
-constexpr int kKwRecord = kKwRows * kKwD + 2 * kKwRows;  // floats: output, maxima, sums
+constexpr uint32_t kKwTmemCols = 512, kKwTmemO = 256;  // S four times 64, O of even steps, O of odd ones
+constexpr int kKwRecord = kKwRows * kKwD + 2 * kKwRows;  // floats: output [dimensions / 4][row][4], maxima, sums
 // f16 x f16 -> f32, both operands K-major
 constexpr uint32_t kw_idesc(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
 
@@ -56,18 +71,30 @@ int read_clear_kv4_wide_error(uint32_t* out) {
 __device__ __forceinline__ void kw_sts128(uint32_t p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(p), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ void kw_sts32(uint32_t p, uint32_t a) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(p), "r"(a) : "memory"); }
+// One thread of a converged warp; operands of what it issues stay in uniform registers.
+__device__ __forceinline__ bool kw_elect() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n selp.u32 %0, 1, 0, e;\n}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void kw_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void kw_st32(uint32_t taddr, const float (&v)[32]) {
-  uint32_t r[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
+// O's next 16 columns of this thread's lane, times f.
+__device__ __forceinline__ void kw_scale16(uint32_t taddr, float f) {
+  uint32_t r[16];
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -83,11 +110,14 @@ __global__ void __launch_bounds__(kKwThreads, 1) k_kv4_attn_wide(const __grid_co
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   __shared__ int cum[kKaListMax + 1];
   __shared__ KaPos place[2];
-  __shared__ uint64_t full[kKwStages], empty[kKwStages], kv_full[2], s_full[2], p_full[2], pv_done[2], begun[2], ended[2], q_ready, drained;
+  __shared__ uint64_t full[kKwStages], empty[kKwStages], k_full[kKwBufs], k_free[kKwBufs], v_full[kKwBufs],
+      v_free[kKwBufs], s_full[4], s_free[4], p_full[2], pv_done[2], begun[2], ended[2], q_ready, drained, met;
   __shared__ uint32_t present[kKwStages];  // pages of the stage that were copied
-  __shared__ uint32_t step_rows[2];        // 16-row pieces of the step that are there
-  __shared__ uint32_t nan_any[2];          // a byte per V warp
-  __shared__ __align__(16) uint8_t nan_row[2][4][kKwStep];  // per V warp (two groups of 16 dimensions) and cache row
+  __shared__ uint32_t step_rows[8];        // by step % 8: its 16-row pieces that are there (operands are made at most 5 steps
+                                   // ahead of the last P, so no slot is written before it was read)
+  __shared__ uint32_t nan_any[kKwBufs];          // a byte per V warp
+  __shared__ __align__(16) uint8_t nan_row[kKwBufs][4][kKwStep];  // per 32 dimensions (a bit per group of 16) and cache row
+  __shared__ float4 row_state[2][kKwRows];  // per group of softmax warps and query row: maximum, sum, NaN groups
   __shared__ uint32_t flags[2], tmem_at;
   volatile uint32_t* abort = flags;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -99,20 +129,29 @@ __global__ void __launch_bounds__(kKwThreads, 1) k_kv4_attn_wide(const __grid_co
       tc_mbar_init(&empty[s], 8);
     }
     for (int s = 0; s < 2; ++s) {
-      tc_mbar_init(&kv_full[s], 8);
-      tc_mbar_init(&s_full[s], 1);
       tc_mbar_init(&p_full[s], 4);
       tc_mbar_init(&pv_done[s], 1);
       tc_mbar_init(&begun[s], 1);
-      tc_mbar_init(&ended[s], 13);
+      tc_mbar_init(&ended[s], 18);
+    }
+    for (int s = 0; s < 4; ++s) {
+      tc_mbar_init(&s_full[s], 2);
+      tc_mbar_init(&s_free[s], 4);
+    }
+    for (int s = 0; s < kKwBufs; ++s) {
+      tc_mbar_init(&k_full[s], 4);
+      tc_mbar_init(&k_free[s], 1);
+      tc_mbar_init(&v_full[s], 4);
+      tc_mbar_init(&v_free[s], 1);
       nan_any[s] = 0;
     }
-    tc_mbar_init(&q_ready, 4);
-    tc_mbar_init(&drained, 1);
+    tc_mbar_init(&q_ready, 8);
+    tc_mbar_init(&met, 8);
+    tc_mbar_init(&drained, 2);
     flags[0] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (tid < 2 * 4 * kKwStep / 4) reinterpret_cast<uint32_t*>(nan_row)[tid] = 0;
+  if (tid < kKwBufs * 4 * kKwStep / 4) reinterpret_cast<uint32_t*>(nan_row)[tid] = 0;
   // rows of P that no thread writes are zero for good
   for (int e = tid; e < 2 * kKwPBytes / 16; e += kKwThreads) kw_sts128(base + kKwOffP + e * 16, 0, 0, 0, 0);
   kw_proxy_fence();
@@ -182,49 +221,54 @@ __global__ void __launch_bounds__(kKwThreads, 1) k_kv4_attn_wide(const __grid_co
     for (uint32_t x = f > kKwStages ? f - kKwStages : 0; x < f; ++x)
       tc_wait_err(&full[x % kKwStages], (x / kKwStages) & 1, nullptr, &g_kv4_error);
 
-  } else if (warp == kKwMmaWarp) {
-    // ---- products ----
+  } else if (warp == kKwMmaWarp || warp == kKwPvWarp) {
+    // ---- products: S by one warp, O += P V by another (issuing is what they spend time on) ----
     uint32_t st = 0, asked = 0;  // steps and items with steps so far
     bool ok = true;
     for (uint32_t item = 0; ok; ++item) {
       ok = ka_wait(&begun[item & 1], (item / 2) & 1, abort);
       if (!ok || !place[item & 1].live) break;
       const int steps = (place[item & 1].c1 - place[item & 1].c0) * (kKaChunk / kKwStep);
-      if (steps) {
-        ok = ka_wait(&q_ready, asked & 1, abort);
-        ++asked;
-      }
-      auto scores = [&](uint32_t x) {  // S of step x
-        const uint32_t buf = x & 1;
-        if (!ka_wait(&kv_full[buf], (x >> 1) & 1, abort)) return false;
-        tc_fence_after();
-        if (lane == 0) {
-#pragma unroll
-          for (int kk = 0; kk < kKwD / 16; ++kk)
-            tc_mma(tmem + buf * kKwStep,
-                   umma_desc_sw128(base + (kk / 4) * (kKwQBytes / 2) + (kk % 4) * 32),
-                   umma_desc_sw128(base + kKwOffK + buf * kKwKBytes + (kk / 4) * (kKwKBytes / 2) + (kk % 4) * 32),
-                   kw_idesc(kKwRows, kKwStep), kk > 0);
-          tc_commit(&s_full[buf]);
+      if (warp == kKwMmaWarp) {
+        if (steps) {
+          ok = ka_wait(&q_ready, asked & 1, abort);
+          ++asked;
         }
-        __syncwarp();
-        return true;
-      };
-      if (ok && steps) ok = scores(st);
-      for (int n = 0; n < steps && ok; ++n) {
-        const uint32_t x = st + n, buf = x & 1;
-        if (n + 1 < steps) ok = scores(x + 1);
-        if (ok) ok = ka_wait(&p_full[buf], (x >> 1) & 1, abort);
-        if (!ok) break;
-        tc_fence_after();
-        if (lane == 0) {
+        for (int n = 0; n < steps && ok; ++n) {
+          const uint32_t x = st + n, buf = x % 4, kb = x % kKwBufs;
+          if (x >= 4) ok = ka_wait(&s_free[buf], (x / 4 - 1) & 1, abort);
+          if (ok) ok = ka_wait(&k_full[kb], (x / kKwBufs) & 1, abort);
+          if (!ok) break;
+          tc_fence_after();
+          if (kw_elect()) {
 #pragma unroll
-          for (int kk = 0; kk < kKwStep / 16; ++kk)
-            tc_mma(tmem + kKwTmemO, umma_desc_sw128(base + kKwOffP + buf * kKwPBytes + kk * 32),
-                   umma_desc_sw128(base + kKwOffV + buf * kKwVBytes + kk * 32), kw_idesc(kKwRows, kKwD), n > 0 || kk > 0);
-          tc_commit(&pv_done[buf]);
+            for (int kk = 0; kk < kKwD / 16; ++kk)
+              tc_mma(tmem + buf * kKwStep,
+                     umma_desc_sw128(base + (kk / 4) * (kKwQBytes / 2) + (kk % 4) * 32),
+                     umma_desc_sw128(base + kKwOffK + kb * kKwKBytes + (kk / 4) * (kKwKBytes / 2) + (kk % 4) * 32),
+                     kw_idesc(kKwRows, kKwStep), kk > 0);
+            tc_commit(&s_full[buf]);
+            tc_arrive(&s_full[buf]);  // (step_rows, seen by this thread, with it)
+            tc_commit(&k_free[kb]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+      } else {
+        for (int n = 0; n < steps && ok; ++n) {
+          const uint32_t x = st + n, buf = x & 1, kb = x % kKwBufs;
+          ok = ka_wait(&v_full[kb], (x / kKwBufs) & 1, abort) && ka_wait(&p_full[buf], (x >> 1) & 1, abort);
+          if (!ok) break;
+          tc_fence_after();
+          if (kw_elect()) {
+#pragma unroll
+            for (int kk = 0; kk < kKwStep / 16; ++kk)
+              tc_mma(tmem + kKwTmemO + buf * kKwD, umma_desc_sw128(base + kKwOffP + buf * kKwPBytes + kk * 32),
+                     umma_desc_sw128(base + kKwOffV + kb * kKwVBytes + kk * 32), kw_idesc(kKwRows, kKwD), n > 1 || kk > 0);
+            tc_commit(&pv_done[buf]);
+            tc_commit(&v_free[kb]);
+          }
+          __syncwarp();
+        }
       }
       st += steps;
       __syncwarp();
@@ -251,90 +295,76 @@ __global__ void __launch_bounds__(kKwThreads, 1) k_kv4_attn_wide(const __grid_co
         if (!ok) break;
         const uint32_t ring = base + kKwOffRing + s * kKwStage, have = present[s];
         for (int half = 0; half < kKaChunk / kKwStep && ok; ++half, ++st) {
-          const uint32_t buf = st & 1;
-          if (st >= 2) ok = ka_wait(&pv_done[buf], ((st >> 1) - 1) & 1, abort);
+          const uint32_t buf = st % kKwBufs;
+          if (st >= kKwBufs) ok = ka_wait(is_v ? &v_free[buf] : &k_free[buf], (st / kKwBufs - 1) & 1, abort);
           if (!ok) break;
           if (!is_v) {
-            // four (row, group) units per thread; eight lanes of a phase have eight rows and one group
+            // two rows x 32 dimensions per thread; eight lanes of a phase read eight 16-byte pieces
+            // of different banks: rows are 64 bytes apart, so the piece moves with the row
+            const int c = (w + (lane >> 1)) & 3;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int combo = w * 4 + j, key = (combo & 7) * 8 + (lane & 7), g = (combo >> 3) * 4 + (lane >> 3);
-              const int r = half * kKwStep + key, page = r >> a.pt_log, in = r & (a.pt - 1);
+            for (int j = 0; j < 2; ++j) {
+              const int key = lane + 32 * j, r = half * kKwStep + key, page = r >> a.pt_log, in = r & (a.pt - 1);
               const uint32_t at = ring + page * block;
-              const uint2 code = ka_lds64(at + in * (kKwD / 2) + g * 8);
-              const uint32_t sc = ka_lds8(at + kv4_off_ks(a.pt, kKwD) + in * (kKwD / 16) + g);
-              const uint32_t f2 = e4m3x2_to_h2(sc | (sc << 8));
-              uint32_t h[8];
-              e2m1x8_to_h2(code.x, reinterpret_cast<uint32_t(&)[4]>(h[0]));
-              e2m1x8_to_h2(code.y, reinterpret_cast<uint32_t(&)[4]>(h[4]));
+              const uint4 code = ka_lds128(at + in * (kKwD / 2) + c * 16);
+              const uint32_t sc = ka_lds16(at + kv4_off_ks(a.pt, kKwD) + in * (kKwD / 16) + c * 2);
+              const uint32_t dst = base + kKwOffK + buf * kKwKBytes + (c >> 1) * (kKwKBytes / 2);
+              const uint32_t both = e4m3x2_to_h2(sc), f2[2] = {__byte_perm(both, 0, 0x1010), __byte_perm(both, 0, 0x3232)};
+              const uint32_t words[4] = {code.x, code.y, code.z, code.w};
 #pragma unroll
-              for (int i = 0; i < 8; ++i) h[i] = hmul2_u(h[i], f2);
-              const uint32_t dst = base + kKwOffK + buf * kKwKBytes + (g >> 2) * (kKwKBytes / 2);
-              kw_sts128(kw_at(dst, key, (g & 3) * 2), h[0], h[1], h[2], h[3]);
-              kw_sts128(kw_at(dst, key, (g & 3) * 2 + 1), h[4], h[5], h[6], h[7]);
+              for (int k = 0; k < 4; ++k) {
+                uint32_t h[4];
+                e2m1x8_to_h2(words[k], h);
+                const uint32_t f = f2[k / 2];
+                kw_sts128(kw_at(dst, key, (c & 1) * 4 + k), hmul2_u(h[0], f), hmul2_u(h[1], f), hmul2_u(h[2], f), hmul2_u(h[3], f));
+              }
             }
             if (w == 0 && lane == 0) {
               uint32_t rows = 0;
               for (int u = 0; u < kKwStep / 16; ++u) rows |= (have >> ((half * kKwStep + u * 16) >> a.pt_log) & 1u) << u;
-              step_rows[buf] = rows;
+              step_rows[st % 8] = rows;
             }
           } else {
-            // eight rows x eight dimensions per thread; eight lanes of a phase have eight row octets
-            const int t = w * 32 + lane, ko = t & 7, dimo = t >> 3;
-            uint32_t c8[8], s8[8];
-            bool odd = false;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int r = half * kKwStep + ko * 8 + j, page = r >> a.pt_log, in = r & (a.pt - 1);
-              const uint32_t at = ring + page * block;
-              c8[j] = ka_lds32(at + kv4_off_v(a.pt, kKwD) + in * (kKwD / 2) + dimo * 4);
-              s8[j] = ka_lds8(at + kv4_off_vs(a.pt, kKwD) + in * (kKwD / 16) + dimo / 2);
-              if (!(have >> page & 1u)) s8[j] = 0;
-              odd |= ka_nan_scale(s8[j]);
-            }
+            // a pair of rows x 32 dimensions per thread, transposed a pair at a time; the pieces and
+            // which row of the pair is read first move with the lane, for the banks' sake as above
+            const int c = (w + lane) & 3, swap = lane >> 2 & 1;
+            const int r = half * kKwStep + 2 * lane, page = r >> a.pt_log, in = r & (a.pt - 1);
+            const uint32_t at = ring + page * block, codes = at + kv4_off_v(a.pt, kKwD) + in * (kKwD / 2) + c * 16;
+            const uint4 one = ka_lds128(codes + swap * (kKwD / 2)), two = ka_lds128(codes + (swap ^ 1) * (kKwD / 2));
+            const uint32_t scales = at + kv4_off_vs(a.pt, kKwD) + in * (kKwD / 16) + c * 2;
+            uint32_t s0 = ka_lds16(scales), s1 = ka_lds16(scales + kKwD / 16);
+            if (!(have >> page & 1u)) s0 = s1 = 0;
+            const bool odd = ka_nan_scale(s0 & 0xff) || ka_nan_scale(s0 >> 8) || ka_nan_scale(s1 & 0xff) || ka_nan_scale(s1 >> 8);
             uint8_t* any = reinterpret_cast<uint8_t*>(&nan_any[buf]) + w;
-            const bool before = *any != 0;
-            __syncwarp();
-            if (before || __any_sync(0xffffffffu, odd)) {  // this warp's two groups: note the rows
-              nan_row[buf][w][lane] = nan_row[buf][w][lane + 32] = 0;
-              if (lane == 0) *any = 0;
+            const bool before = *any != 0, now = __any_sync(0xffffffffu, odd);
+            if (before || now) {  // note the rows
+              nan_row[buf][c][2 * lane] = (uint8_t)(ka_nan_scale(s0 & 0xff) | ka_nan_scale(s0 >> 8) << 1);
+              nan_row[buf][c][2 * lane + 1] = (uint8_t)(ka_nan_scale(s1 & 0xff) | ka_nan_scale(s1 >> 8) << 1);
+              if (ka_nan_scale(s0 & 0xff)) s0 &= 0xff00;
+              if (ka_nan_scale(s0 >> 8)) s0 &= 0xff;
+              if (ka_nan_scale(s1 & 0xff)) s1 &= 0xff00;
+              if (ka_nan_scale(s1 >> 8)) s1 &= 0xff;
               __syncwarp();
-              for (int half_group = 0; half_group < 2; ++half_group) {  // (bytes of a row are written by one group at a time)
-                if ((dimo >> 1 & 1) == half_group && !(dimo & 1)) {
-                  for (int j = 0; j < 8; ++j)
-                    if (ka_nan_scale(s8[j])) {
-                      nan_row[buf][w][ko * 8 + j] |= (uint8_t)(1u << half_group);
-                      *any = 1;
-                    }
-                }
-                __syncwarp();
-              }
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (ka_nan_scale(s8[j])) s8[j] = 0;
+              if (lane == 0) *any = now;
             }
-            uint32_t f2[4];
+            // a factor per row of the pair, for each of the two groups
+            const uint32_t fx = e4m3x2_to_h2(s0), fy = e4m3x2_to_h2(s1);
+            const uint32_t f2[2] = {__byte_perm(fx, fy, 0x5410), __byte_perm(fx, fy, 0x7632)};
+            const uint32_t first[4] = {one.x, one.y, one.z, one.w}, second[4] = {two.x, two.y, two.z, two.w};
+            const uint32_t dst = base + kKwOffV + buf * kKwVBytes + c * 32 * 128 + (lane & 3) * 4;
 #pragma unroll
-            for (int p = 0; p < 4; ++p) f2[p] = e4m3x2_to_h2(s8[2 * p] | (s8[2 * p + 1] << 8));
-            const uint32_t dst = base + kKwOffV + buf * kKwVBytes;
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t x = swap ? second[k] : first[k], y = swap ? first[k] : second[k];
+              uint32_t h[2][4];
+              e2m1x8_to_h2((x & 0x0f0f0f0fu) | ((y << 4) & 0xf0f0f0f0u), h[0]);  // even dimensions
+              e2m1x8_to_h2(((x >> 4) & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u), h[1]);  // odd ones
 #pragma unroll
-            for (int par = 0; par < 2; ++par) {  // even and odd dimensions
-              uint32_t h[4][4];
-#pragma unroll
-              for (int p = 0; p < 4; ++p) {
-                const uint32_t x = c8[2 * p], y = c8[2 * p + 1];
-                e2m1x8_to_h2(par == 0 ? (x & 0x0f0f0f0fu) | ((y << 4) & 0xf0f0f0f0u) : ((x >> 4) & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u),
-                             h[p]);
-              }
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                kw_sts128(kw_at(dst, dimo * 8 + 2 * i + par, ko), hmul2_u(h[0][i], f2[0]), hmul2_u(h[1][i], f2[1]),
-                          hmul2_u(h[2][i], f2[2]), hmul2_u(h[3][i], f2[3]));
+              for (int d = 0; d < 8; ++d) kw_sts32(kw_at(dst, k * 8 + d, lane >> 2), hmul2_u(h[d & 1][d >> 1], f2[k / 2]));
             }
           }
           kw_proxy_fence();
           __syncwarp();
-          if (lane == 0) tc_arrive(&kv_full[buf]);
+          if (lane == 0) tc_arrive(is_v ? &v_full[buf] : &k_full[buf]);
         }
         __syncwarp();
         if (ok && lane == 0) tc_arrive(&empty[s]);
@@ -344,10 +374,10 @@ __global__ void __launch_bounds__(kKwThreads, 1) k_kv4_attn_wide(const __grid_co
     }
 
   } else {
-    // ---- a query row per thread ----
-    const int r = tid;
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-    uint32_t st = 0;
+    // ---- a query row per thread, even steps by warps 0..3 and odd ones by warps 4..7 ----
+    const int grp = warp >> 2, r = tid & (kKwRows - 1);
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    uint32_t st = 0, meetings = 0;  // steps and meetings of the two groups so far
     bool ok = true;
     for (uint32_t item = 0; ok; ++item) {
       ok = ka_wait(&begun[item & 1], (item / 2) & 1, abort);
@@ -364,23 +394,23 @@ __global__ void __launch_bounds__(kKwThreads, 1) k_kv4_attn_wide(const __grid_co
         // q as f16, scaled per row by a power of two
         const uint4* q = reinterpret_cast<const uint4*>(a.q + ((int64_t)it.b * a.T + i) * a.q_stride +
                                                         (int64_t)(it.h * a.G + row - i * a.G) * kKwD);
+        uint4 v[kKwD / 8];
+#pragma unroll
+        for (int c = 0; c < kKwD / 8; ++c) v[c] = live ? q[c ^ (8 * grp)] : make_uint4(0, 0, 0, 0);  // own half first
         uint32_t mx = 0;
-#pragma unroll 4
-        for (int c = 0; c < kKwD / 8; ++c) {
-          const uint4 v = live ? q[c] : make_uint4(0, 0, 0, 0);
-          mx = __vmaxu2(__vmaxu2(mx, v.x & 0x7fff7fffu), __vmaxu2(v.y & 0x7fff7fffu, __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
-        }
+#pragma unroll
+        for (int c = 0; c < kKwD / 8; ++c)
+          mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(v[c].x & 0x7fff7fffu, v[c].y & 0x7fff7fffu),
+                                     __vmaxu2(v[c].z & 0x7fff7fffu, v[c].w & 0x7fff7fffu)));
         float undo;
         float mul = ka_q_scale(max(mx & 0xffffu, mx >> 16), &undo);
         sc = fmaxf(a.scale_log2 * undo, 1e-37f);  // never 0: 0 x -inf
         if (a.negate) mul = -mul;
-#pragma unroll 4
-        for (int c = 0; c < kKwD / 8; ++c) {
-          const uint4 v = live ? q[c] : make_uint4(0, 0, 0, 0);
-          kw_sts128(kw_at(base + (c / 8) * (kKwQBytes / 2), r, c % 8), ka_h2(bf_lo(v.x) * mul, bf_hi(v.x) * mul),
-                    ka_h2(bf_lo(v.y) * mul, bf_hi(v.y) * mul), ka_h2(bf_lo(v.z) * mul, bf_hi(v.z) * mul),
-                    ka_h2(bf_lo(v.w) * mul, bf_hi(v.w) * mul));
-        }
+#pragma unroll
+        for (int c = 0; c < kKwD / 16; ++c)
+          kw_sts128(kw_at(base + grp * (kKwQBytes / 2), r, c), ka_h2(bf_lo(v[c].x) * mul, bf_hi(v[c].x) * mul),
+                    ka_h2(bf_lo(v[c].y) * mul, bf_hi(v[c].y) * mul), ka_h2(bf_lo(v[c].z) * mul, bf_hi(v[c].z) * mul),
+                    ka_h2(bf_lo(v[c].w) * mul, bf_hi(v[c].w) * mul));
         kw_proxy_fence();
         __syncwarp();
         if (lane == 0) tc_arrive(&q_ready);
@@ -390,18 +420,22 @@ __global__ void __launch_bounds__(kKwThreads, 1) k_kv4_attn_wide(const __grid_co
       const int all_hi = it.x.pos + it.x.t0, all_lo = a.window > 0 ? it.x.pos + it.x.t1 - a.window + 1 : 0;
       const int sink_chunks = it.x.sink_chunks, lo_chunk = it.x.lo_chunk;
       const int steps = (c1 - c0) * (kKaChunk / kKwStep);
-      for (int n = 0; n < steps && ok; ++n, ++st) {
-        const uint32_t buf = st & 1, phase = (st >> 1) & 1;
-        ok = ka_wait(&kv_full[buf], phase, abort) && ka_wait(&s_full[buf], phase, abort);
+      // (an item has an even number of steps, so a group's steps use one buffer: its own)
+      for (int n = grp; n < steps && ok; n += 2) {
+        const uint32_t x = st + n, buf = grp, kb = x % kKwBufs;
+        ok = ka_wait(&s_full[x % 4], (x >> 2) & 1, abort);
         if (!ok) break;
         tc_fence_after();
         if (busy) {
+          const uint32_t rows = step_rows[x % 8];
+          float s[kKwStep];
+          tc_ld32(lanes + x % 4 * kKwStep, reinterpret_cast<float(&)[32]>(s[0]));
+          tc_ld32(lanes + x % 4 * kKwStep + 32, reinterpret_cast<float(&)[32]>(s[32]));
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc_arrive(&s_free[x % 4]);
           const int c = c0 + n / 2;
           const int key0 = (c < sink_chunks ? c : lo_chunk + c - sink_chunks) * kKaChunk + (n & 1) * kKwStep;
-          const uint32_t rows = step_rows[buf];
-          float s[kKwStep];
-          tc_ld32(lanes + buf * kKwStep, reinterpret_cast<float(&)[32]>(s[0]));
-          tc_ld32(lanes + buf * kKwStep + 32, reinterpret_cast<float(&)[32]>(s[32]));
           auto see = [&](int e) {
             const int key = key0 + e;
             return key <= rowpos && (a.window == 0 || key > rowpos - a.window || key < a.sinks) && (rows >> (e / 16) & 1u);
@@ -411,58 +445,63 @@ __global__ void __launch_bounds__(kKwThreads, 1) k_kv4_attn_wide(const __grid_co
             for (int e = 0; e < kKwStep; ++e)
               if (!see(e)) s[e] = -INFINITY;
           }
-          if (nan_any[buf] != 0) {
-            for (int e = 0; e < kKwStep; ++e)
-              if (see(e))
-                for (int x = 0; x < 4; ++x) nan_groups |= (uint32_t)nan_row[buf][x][e] << (2 * x);
-          }
-          float top = s[0];
+          float tops[8];
 #pragma unroll
-          for (int e = 1; e < kKwStep; ++e) top = fmaxf(top, s[e]);
-          top *= sc;
+          for (int e = 0; e < 8; ++e) tops[e] = s[e];
+#pragma unroll
+          for (int e = 8; e < kKwStep; ++e) tops[e % 8] = fmaxf(tops[e % 8], s[e]);
+          const float top = sc * fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
+                                       fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
           const bool move = top > m + kKaLazy;
           if (__any_sync(0xffffffffu, move)) {
             const float f = !move ? 1.f : m == -INFINITY ? 0.f : ka_exp2(m - top);
             if (move) m = top;
             l *= f;
-            if (n > 0) {  // O of the steps before is complete, and nothing adds to it until P is handed over
-              ok = ka_wait(&pv_done[(st - 1) & 1], ((st - 1) >> 1) & 1, abort);
+            if (n > 1) {  // this group's O is complete, and nothing adds to it until P is handed over
+              ok = ka_wait(&pv_done[buf], ((x >> 1) - 1) & 1, abort);
               if (!ok) break;
               tc_fence_after();
 #pragma unroll 1
-              for (int x = 0; x < kKwD / 32; ++x) {
-                float v[32];
-                tc_ld32(lanes + kKwTmemO + x * 32, v);
-#pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] *= f;
-                kw_st32(lanes + kKwTmemO + x * 32, v);
-              }
+              for (int y = 0; y < kKwD; y += 16) kw_scale16(lanes + kKwTmemO + buf * kKwD + y, f);
             }
           }
           const float ref = m == -INFINITY ? 0.f : kKaOff - m;
+          if (x >= 2) ok = ka_wait(&pv_done[buf], ((x >> 1) - 1) & 1, abort);
+          if (!ok) break;
           float sum[2] = {0.f, 0.f};
-          uint32_t p2[kKwStep / 2];
 #pragma unroll
-          for (int e = 0; e < kKwStep; e += 2) {
-            const float x = ka_exp2(__fmaf_rn(s[e], sc, ref)), y = ka_exp2(__fmaf_rn(s[e + 1], sc, ref));
-            sum[0] += x;
-            sum[1] += y;
-            p2[e / 2] = ka_h2(x, y);
+          for (int y = 0; y < kKwStep / 8; ++y) {
+            uint32_t p2[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float w0 = ka_exp2(__fmaf_rn(s[8 * y + 2 * e], sc, ref)), w1 = ka_exp2(__fmaf_rn(s[8 * y + 2 * e + 1], sc, ref));
+              sum[0] += w0;
+              sum[1] += w1;
+              p2[e] = ka_h2(w0, w1);
+            }
+            kw_sts128(kw_at(base + kKwOffP + buf * kKwPBytes, r, y), p2[0], p2[1], p2[2], p2[3]);
           }
           l += sum[0] + sum[1];
-          if (st >= 2) ok = ka_wait(&pv_done[buf], ((st >> 1) - 1) & 1, abort);
+          ok = ka_wait(&v_full[kb], (x / kKwBufs) & 1, abort);
           if (!ok) break;
-#pragma unroll
-          for (int x = 0; x < kKwStep / 8; ++x)
-            kw_sts128(kw_at(base + kKwOffP + buf * kKwPBytes, r, x), p2[4 * x], p2[4 * x + 1], p2[4 * x + 2], p2[4 * x + 3]);
+          if (nan_any[kb] != 0) {
+            for (int e = 0; e < kKwStep; ++e)
+              if (see(e))
+                for (int y = 0; y < 4; ++y) nan_groups |= (uint32_t)nan_row[kb][y][e] << (2 * y);
+          }
           kw_proxy_fence();
+        } else {
+          if (lane == 0) tc_arrive(&s_free[x % 4]);
+          if (x >= 2) ok = ka_wait(&pv_done[buf], ((x >> 1) - 1) & 1, abort);  // (or P's arrival could count for the step before)
+          if (!ok) break;
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) tc_arrive(&p_full[buf]);
       }
+      st += steps;
       if (!ok) break;
-      // ---- the item's end: O out of TMEM ----
+      // ---- the item's end: the groups' states meet, O out of TMEM, half of the dimensions each ----
       const bool whole = c1 - c0 == it.x.n;
       const int u0 = it.w - c0;
       int first = blockIdx.x, parts = 1;
@@ -472,48 +511,73 @@ __global__ void __launch_bounds__(kKwThreads, 1) k_kv4_attn_wide(const __grid_co
       }
       const int odd = !whole && ka_range(it, first) < u0;
       if (tid == 0 && c0 == 0) info[((int64_t)it.b * a.nkv + it.h) * a.tiles + it.tile] = {first, parts, odd, 0};
+      float weight[2] = {0.f, 0.f};
       if (steps) {
-        ok = ka_wait(&pv_done[(st - 1) & 1], ((st - 1) >> 1) & 1, abort);
+        row_state[grp][r] = make_float4(m, l, __uint_as_float(nan_groups), 0.f);
+        __syncwarp();
+        if (lane == 0) tc_arrive(&met);
+        ok = ka_wait(&met, meetings++ & 1, abort) && ka_wait(&pv_done[0], ((st - 2) >> 1) & 1, abort) &&
+             ka_wait(&pv_done[1], ((st - 1) >> 1) & 1, abort);
         if (!ok) break;
         tc_fence_after();
+        const float4 other = row_state[grp ^ 1][r];
+        const float to = fmaxf(m, other.x);
+        weight[grp] = m == -INFINITY ? 0.f : ka_exp2(m - to);
+        weight[grp ^ 1] = other.x == -INFINITY ? 0.f : ka_exp2(other.x - to);
+        l = l * weight[grp] + other.y * weight[grp ^ 1];
+        m = to;
+        nan_groups |= __float_as_uint(other.z);
       }
       float* rec = a.parts + (size_t)(2 * blockIdx.x + (blockIdx.x == (unsigned)first ? odd : 0)) * kKwRecord;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       if (busy) {
 #pragma unroll 1
-        for (int x = 0; x < kKwD / 32; ++x) {
+        for (int x = 2 * grp; x < 2 * grp + 2; ++x) {
           float v[32];
-          if (steps) {
-            tc_ld32(lanes + kKwTmemO + x * 32, v);
-          } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = 0.f;
+          for (int e = 0; e < 32; ++e) v[e] = 0.f;
+          if (steps) {
+#pragma unroll 1
+            for (int y = 0; y < 2; ++y) {
+              float o[32];
+              tc_ld32(lanes + kKwTmemO + y * kKwD + x * 32, o);
+              const float f = weight[y];
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] += o[e] * f;
+            }
           }
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (nan_groups >> (2 * x + e / 16) & 1u) v[e] = NAN;
-          if (!live) continue;
-          if (whole) {
+          if (live && whole) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = on ? v[e] * inv : 0.f;
 #pragma unroll
             for (int e = 0; e < 32; e += 8)
               *reinterpret_cast<uint4*>(out + x * 32 + e) =
                   make_uint4(pack2(v[e], v[e + 1]), pack2(v[e + 2], v[e + 3]), pack2(v[e + 4], v[e + 5]), pack2(v[e + 6], v[e + 7]));
-          } else {
+          } else if (live) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(rec + r * kKwD + x * 32 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+              *reinterpret_cast<float4*>(rec + ((x * 32 + e) / 4 * kKwRows + r) * 4) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
           }
+          __syncwarp();
         }
-        if (!whole && live) {
+        if (!whole && live && grp == 0) {
           rec[kKwRows * kKwD + r] = m;
           rec[kKwRows * kKwD + kKwRows + r] = l;
         }
       }
+      // both groups have read both halves of O before either hands over the next item's first P
       tc_fence_before();
       __syncwarp();
+      if (steps) {
+        if (lane == 0) tc_arrive(&met);
+        ok = ka_wait(&met, meetings++ & 1, abort);
+        if (!ok) break;
+      }
       if (lane == 0) tc_arrive(&ended[item & 1]);
+      __syncwarp();
     }
     // rows of items without a chunk
     if (a.listed) {
@@ -523,7 +587,7 @@ __global__ void __launch_bounds__(kKwThreads, 1) k_kv4_attn_wide(const __grid_co
         if (ka_tile(a, b, tile).n) continue;
         if (tid == 0) info[k] = {0, 1, 0, 0};
         const int row = tile * kKwRows + r, i = ka_div_g(a, row);
-        if (row < a.G * a.T)
+        if (row < a.G * a.T && grp == 0)
           for (int d = 0; d < kKwD; d += 8)
             *reinterpret_cast<uint4*>(a.out + ((int64_t)b * a.T + i) * a.out_stride + (int64_t)(h * a.G + row - i * a.G) * kKwD + d) =
                 make_uint4(0u, 0u, 0u, 0u);
@@ -552,6 +616,17 @@ __global__ void __launch_bounds__(kKjThreads) k_kv4_join(const __grid_constant__
   if (x.parts <= 1 || x.first < 0 || x.parts > ctas || x.first > ctas - x.parts || tile * kKwRows + r0 >= a.G * a.T) return;
   auto record = [&](int p) { return a.parts + (size_t)(2 * (x.first + p) + (p == 0 && x.odd ? 1 : 0)) * kKwRecord; };
   const int row = tid % kKjRows, p0 = tid / kKjRows, step = kKjThreads / kKjRows;
+  constexpr int kMine = kKjRows * kKwD / 4 / kKjThreads;
+  float4 v[kMine][4];
+  auto load = [&](int q) {  // four parts of this thread's pieces (the last one again where there are fewer)
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const float4* rec = reinterpret_cast<const float4*>(record(min(q + p, x.parts - 1))) + r0 + row;
+#pragma unroll
+      for (int k = 0; k < kMine; ++k) v[k][p] = rec[(p0 + k * step) * kKwRows];
+    }
+  };
+  load(0);
   float top = -INFINITY;
   for (int p = p0; p < x.parts; p += step) {
     const float m = record(p)[kKwRows * kKwD + r0 + row];
@@ -571,36 +646,28 @@ __global__ void __launch_bounds__(kKjThreads) k_kv4_join(const __grid_constant__
   }
   part_sum[tid] = sum;
   __syncthreads();
-  constexpr int kMine = kKjRows * kKwD / 4 / kKjThreads;
   float4 acc[kMine];
 #pragma unroll
   for (int k = 0; k < kMine; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int q = 0; q < x.parts; q += 4) {
-    float4 v[kMine][4];
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const float4* rec = reinterpret_cast<const float4*>(record(min(q + p, x.parts - 1)) + r0 * kKwD);
-#pragma unroll
-      for (int k = 0; k < kMine; ++k) v[k][p] = rec[tid + k * kKjThreads];
-    }
+    if (q) load(q);
 #pragma unroll
     for (int p = 0; p < 4; ++p)
       if (q + p < x.parts)
 #pragma unroll
         for (int k = 0; k < kMine; ++k) {
-          const float f = wgt[(q + p) * kKjRows + (tid + k * kKjThreads) / (kKwD / 4)];
+          const float f = wgt[(q + p) * kKjRows + row];
           acc[k] = make_float4(acc[k].x + v[k][p].x * f, acc[k].y + v[k][p].y * f, acc[k].z + v[k][p].z * f, acc[k].w + v[k][p].w * f);
         }
   }
   const int used = a.n_tokens ? min(max(a.n_tokens[b], 0), a.T) : a.T;
 #pragma unroll
   for (int k = 0; k < kMine; ++k) {
-    const int e = tid + k * kKjThreads, r = e / (kKwD / 4), d = e % (kKwD / 4) * 4;
-    const int query = tile * kKwRows + r0 + r, i = ka_div_g(a, query);
+    const int d = (p0 + k * step) * 4, query = tile * kKwRows + r0 + row, i = ka_div_g(a, query);
     if (query >= a.G * a.T) continue;
     float l = 0.f;
 #pragma unroll
-    for (int y = 0; y < kKjThreads / kKjRows; ++y) l += part_sum[y * kKjRows + r];
+    for (int y = 0; y < kKjThreads / kKjRows; ++y) l += part_sum[y * kKjRows + row];
     const float f = l == 0.f || i >= used ? 0.f : 1.f / l;
     uint2 o = make_uint2(pack2(acc[k].x * f, acc[k].y * f), pack2(acc[k].z * f, acc[k].w * f));
     if (i >= used) o = make_uint2(0u, 0u);

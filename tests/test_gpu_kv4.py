@@ -327,6 +327,103 @@ def test_attention_long_and_unequal(jsx, cuda, B, T, nq, nkv, L):
     attn_case(jsx, rng, B, T, nq, nkv, 128, 64, positions)
 
 
+# ---- many query rows: a table with room for long sequences takes the kernel of 128-row items ----
+
+
+@pytest.mark.parametrize("T,nq,nkv,pt,counts", [(4, 32, 2, 64, False), (5, 32, 2, 128, False), (7, 14, 2, 32, False),
+                                                (8, 16, 1, 16, False), (16, 32, 2, 64, True), (33, 12, 4, 32, True),
+                                                (70, 16, 1, 64, True), (300, 1, 1, 16, False)])
+def test_attention_many_rows(jsx, cuda, T, nq, nkv, pt, counts):
+    rng = np.random.default_rng(T + nq)
+    positions = [0, 60, 331, -T + 1, -T]
+    attn_case(jsx, rng, 5, T, nq, nkv, 128, pt, positions, n_tokens=[T, T - 1, T, 0, T] if counts else None,
+              slots=2 ** 18 // pt)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (33, 5), (130, 200), (1000, 3)])
+def test_attention_many_rows_window_and_sinks(jsx, cuda, window, sinks):
+    rng = np.random.default_rng(window)
+    attn_case(jsx, rng, 4, 240, 16, 2, 128, 32, [0, 63, 300, 777], window=window, sinks=sinks, slots=512)
+
+
+@pytest.mark.parametrize("B,T,nq,nkv,L", [(3, 8, 32, 2, 5000), (2, 16, 16, 1, 9000), (1, 64, 32, 2, 2000)])
+def test_attention_many_rows_long_and_unequal(jsx, cuda, B, T, nq, nkv, L):
+    """The same item's records of many CTAs, long sequences in few of them."""
+    rng = np.random.default_rng(L)
+    positions = [L - 1 if b == 0 else int(rng.integers(0, max(2, L // 20))) for b in range(B)]
+    attn_case(jsx, rng, B, T, nq, nkv, 128, 64, positions, slots=4096)
+
+
+def test_attention_many_rows_missing_pages(jsx, cuda):
+    def holes(t):
+        t = t.copy()
+        t[0, 1] = -1
+        t[1, :] = -1          # nothing left: zeros
+        t[2, 0] = 10 ** 6     # not a page
+        return t
+    rng = np.random.default_rng(8)
+    out = attn_case(jsx, rng, 4, 8, 32, 2, 128, 16, [200, 70, 130, 500], table=holes, slots=2048)
+    assert (out.view(4, 8, -1)[1] == 0).all()
+
+
+def test_attention_many_rows_nan_that_only_some_tokens_see(jsx, cuda):
+    """V rows with a NaN that the later tokens see, a K row with one that the last token sees."""
+    rng = np.random.default_rng(16)
+    T, nq, first, pt = 16, 16, 250, 32
+    t, pages = make_table(rng, [300], pt, 2 ** 18 // pt)
+    k, v = rows(rng, 1, 300, 1, 128), rows(rng, 1, 300, 1, 128)
+    q = rows(rng, T, nq * 128)
+    ws = jsx.kernels.kv4_attn_workspace(1, T, nq, 1, 128, q.device)
+
+    def run(kk, vv):
+        pool = make_pool(jsx, pages, 1, 128, pt)
+        jsx.kernels.kv4_append(kk, vv, pool, dev(t), dev([0]), tokens_per_seq=300)
+        return jsx.kernels.kv4_attn(q, pool, dev(t), dev([first]), 128, ws, tokens_per_seq=T).view(T, nq, 128)
+
+    clean = run(k, v)
+    assert torch.isfinite(clean.float()).all()
+    vv = v.clone()
+    vv[0, first + 3, 0, 17] = float("nan")
+    vv[0, first + 10, 0, 127] = float("nan")
+    vv[0, first + T, 0, 64] = float("nan")      # after the last token: no one's
+    o = run(k, vv)
+    want = torch.zeros(T, nq, 128, dtype=torch.bool, device="cuda")
+    want[3:, :, 16:32] = True
+    want[10:, :, 112:] = True
+    assert torch.equal(torch.isnan(o), want) and torch.equal(o[~want], clean[~want])
+    assert torch.equal(run(k, v), clean)        # and nothing of it stays
+    kk = k.clone()
+    kk[0, first + T - 1, 0, 3] = float("nan")
+    o = run(kk, v)
+    assert torch.isnan(o[T - 1]).all() and torch.equal(o[:T - 1], clean[:T - 1])
+
+
+@pytest.mark.parametrize("T,nq", [(1, 4), (4, 16)])
+def test_attention_many_sequences(jsx, cuda, T, nq):
+    """More sequences than the list of chunks is kept for: whole items per CTA."""
+    rng = np.random.default_rng(T)
+    positions = [int(x) for x in rng.integers(-T, 300, 600)]
+    attn_case(jsx, rng, 600, T, nq, 1, 128, 32, positions, slots=16)
+
+
+def test_attention_workspace_of_the_largest_call(jsx, cuda):
+    """One workspace, calls of several shapes in turn: each as with a workspace of its own."""
+    rng = np.random.default_rng(21)
+    B, hd, pt = 3, 128, 64
+    t, pages = make_table(rng, [3000] * B, pt, 2048)
+    pool = make_pool(jsx, pages, 2, hd, pt)
+    k, v = rows(rng, B, 3000, 2, hd), rows(rng, B, 3000, 2, hd)
+    jsx.kernels.kv4_append(k, v, pool, dev(t), dev([0] * B), tokens_per_seq=3000)
+    tab, pos = dev(t), dev([2900, 17, 1500])
+    shared = jsx.kernels.kv4_attn_workspace(B, 16, 32, 2, hd, pool.device)
+    for T in (16, 1, 8, 2, 16, 1):
+        q = rows(rng, B * T, 32 * hd)
+        own = jsx.kernels.kv4_attn_workspace(B, T, 32, 2, hd, pool.device)
+        assert own.numel() <= shared.numel()
+        a = jsx.kernels.kv4_attn(q, pool, tab, pos, hd, own, tokens_per_seq=T)
+        assert torch.equal(a, jsx.kernels.kv4_attn(q, pool, tab, pos, hd, shared, tokens_per_seq=T))
+
+
 def test_attention_strided_queries_another_stream_and_graph(jsx, cuda):
     rng = np.random.default_rng(11)
     B, T, nq, nkv, hd, pt = 4, 2, 8, 2, 128, 32
