@@ -351,7 +351,7 @@ __device__ __forceinline__ unsigned long long vf_scan(unsigned long long x) {  /
   return x;
 }
 
-// By one CTA per sequence: the draw, the outputs, and the rows' records zero again.
+// By one CTA per sequence: the draw, the outputs, and the workspace zero again.
 template <typename E>
 __device__ __forceinline__ void vf_pick(const VfArgs& a, int b, const VfSeq& s, float prob, float u) {
   __shared__ unsigned long long warps[kVfWarps], reached;
@@ -420,6 +420,7 @@ __device__ __forceinline__ void vf_pick(const VfArgs& a, int b, const VfSeq& s, 
         token = draw.vec.first(j) + e;
       }
     }
+    for (int k = tid; k < n; k += kVfThreads) steps[k] = 0;  // (the next call's records may lie here)
   }
   __syncthreads();
   if (tid <= T) {
@@ -427,9 +428,7 @@ __device__ __forceinline__ void vf_pick(const VfArgs& a, int b, const VfSeq& s, 
     if (tid < s.accepted) t = a.ids[(int64_t)b * T + tid];
     if (tid == s.accepted) t = token;
     a.tokens[(int64_t)b * (T + 1) + tid] = t;
-    VfRow* r = a.rows + (int64_t)b * (T + 1) + tid;
-    r->sum = 0;
-    r->top = r->best = r->arrived = 0;
+    a.rows[(int64_t)b * (T + 1) + tid] = VfRow{};
   }
 }
 

@@ -447,8 +447,9 @@ int jsx_kv4_read(const void* pool, int num_pages, const int32_t* page_table, int
  * j < sinks); out = softmax(scale q.k) v over the visible rows, 0 when there is
  * none.  q and out [B * T][nq][head_dim] bf16 with token strides q_stride and
  * out_stride (elements, multiples of 8); query head h reads kv head h / (nq / nkv).
- * workspace: jsx_kv4_attn_workspace_size bytes, 16-byte aligned, zero-filled once
- * (left zeroed by every call). */
+ * workspace: jsx_kv4_attn_workspace_size bytes, 16-byte aligned, zero-filled once.
+ * Calls of other shapes that follow one another may share the largest one's; calls
+ * that run at the same time may not. */
 int jsx_kv4_attn_workspace_size(int B, int T, int nq, int nkv, int head_dim, size_t* bytes);
 int jsx_kv4_attn(const void* q, int64_t q_stride, const void* pool, int num_pages,
                  const int32_t* page_table, int table_slots, const int32_t* positions,
@@ -502,7 +503,8 @@ int jsx_pages_compact(const int32_t* table, const int32_t* held, const int32_t* 
  * depend on the order of execution.  NaN logits have no mass; a row without a
  * finite maximum accepts nothing and draws -1.  0 <= T <= 31, V <= 2^20,
  * B (T + 1) <= 65535.  workspace: jsx_verify_workspace_size bytes, 16-byte aligned,
- * zero-filled once (left so that the next call can use it). */
+ * zero-filled once and zero again after every call: calls of other shapes that follow
+ * one another may share the largest one's, calls that run at the same time may not. */
 int jsx_verify_workspace_size(int B, int T, int V, size_t* bytes);
 int jsx_verify_drafts(const void* logits, int logits_f32, int64_t row_stride,
                       const int32_t* draft_ids, const float* draft_probs, const int32_t* n_draft,

@@ -138,6 +138,22 @@ def test_strided_rows_of_logits(jsx, cuda):
         assert torch.equal(s, t)
 
 
+def test_one_workspace_for_calls_of_several_shapes(jsx, cuda):
+    """Records of one shape lie where another shape keeps its sums: every call leaves zeros."""
+    rng = np.random.default_rng(31)
+    shapes = [(2, 31, 257), (40, 0, 9001), (9, 4, 3001), (2, 31, 257), (1, 2, 151552), (40, 0, 9001)]
+    size = max(jsx.kernels.verify_workspace(B, T, V, torch.device("cuda")).numel() for B, T, V in shapes)
+    shared = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    for B, T, V in shapes:
+        for temperature in (1.0, 0.0):
+            x, ids, u, q = make(rng, B, T, V, probs=T > 2, temperature=temperature)
+            own = jsx.kernels.verify_workspace(B, T, V, x.device)
+            a = jsx.kernels.verify_drafts(x, ids, u, own, draft_probs=q, temperature=temperature)
+            b = jsx.kernels.verify_drafts(x, ids, u, shared, draft_probs=q, temperature=temperature)
+            assert all(torch.equal(y, z) for y, z in zip(a, b))
+            assert not shared.any()
+
+
 def test_refusals(jsx, cuda):
     K = jsx.kernels
     x = torch.zeros(2, 3, 100, device="cuda")
