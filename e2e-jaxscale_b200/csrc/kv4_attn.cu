@@ -24,6 +24,15 @@
 // (V) pieces of a row: lane t of a quad holds dimensions t D/4 .. of a K row, column c of O
 // stands for dimensions c D/8 .. .  For P V, whose operand pairs two rows, the nibbles
 // of two rows are interleaved before they are converted.
+//
+// Bound: not the bytes but the mix of conversions, multiplications and MMAs of 16 cache rows x
+// 16 query rows, which share the schedulers: two mma.sync (18.8 cycles of a scheduler alone),
+// four conversions (12.8) and four hmul2 (8.3) take 27 together, the loop runs at 88% of that.
+// 32 sequences of up to 32768 rows, 32 heads on 2: 69 us = 2.8 TB/s of the pages, 0.43 of the
+// copy rate; 64 sequences with a window of 4096: 27.5 us; one sequence of 1025 rows: 10.9 us,
+// latency of a chain of place, pages, product and join.  Measured and not taken: three CTAs
+// per SM of 128 registers (73 us), one of twelve warps with 16-row pieces (75), copies issued
+// by a computing warp (106).
 #include <math.h>
 
 #include "kv4_attn.cuh"

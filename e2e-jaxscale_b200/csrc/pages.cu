@@ -17,8 +17,11 @@
 // them without further launches.  Ranks are prefix sums over page and sequence
 // order, so the pages chosen do not depend on the order of execution.  Page
 // bytes move in a second launch, one (page, layer) unit per CTA at a time,
-// reading the page list that the first one wrote; both halves are bound by
-// memory (2 x the copied bytes) once there is more than a few megabytes to move.
+// reading the page list that the first one wrote.  Bound: the copy by memory once there is
+// more than a few megabytes to move (500 pages of 40 layers, 737 MB read and written: 128 us
+// with the bookkeeping, 0.88 of the copy rate; one load of a page in flight at a time: 147 us),
+// the bookkeeping by its chain of barriers and loads (forking one row into 4: 8.6 us,
+// 8 into 64 with growth and the copies: 27 us).
 #include "common.cuh"
 #include "launch.cuh"
 
