@@ -21,11 +21,12 @@
 // CTA of a sequence finds the step with the crossing and weighs it again.  Slices meet in
 // integer atomics (maximum, sum), so they need no order and no wait; the second pass
 // over the logits comes from L2 (at most 126 MB of it).  At temperature 0 (greedy: p is
-// 1 at the lowest index of the maximum) nothing is weighed.
+// 1 at the lowest index of the maximum) nothing is weighed, and one launch does it all.
 // Bound: from some 20 rows on the exponentials' instructions (18 per logit with the exact
 // sum, 75% of the issue slots) rather than the bytes; launches below.  32 x 5 rows of 151552
 // with draft distributions: 44 us, 12 of them the maxima (4.0 TB/s) and 21 the sums; 1 x 5:
-// 13.5 us; 16 x 8 rows of 32003, greedy: 7.9 us.  One cluster per row with distributed
+// 13.5 us; 16 x 8 rows of 32003, greedy: 5.8 us (7.9 in three launches, which also cost the
+// host 5 us more).  One cluster per row with distributed
 // shared memory instead of atomics: 79 us.
 // NaN logits and a row's -inf entries have no mass; a row with no mass at all, or
 // with +inf, accepts nothing and draws token -1 (greedy takes +inf as the maximum).
@@ -43,14 +44,20 @@ constexpr int kVfMaxVocab = 1 << 20;
 constexpr int kVfMaxPer = 8;  // vectors a thread weighs before its warp adds them up (32 bits hold 15 x 8 x 32 x 2^20)
 
 // Per (sequence, position).  Zero between calls: the slices add and take maxima.
-struct VfRow {
-  unsigned long long sum;  // Z; 0: no distribution
+struct __align__(16) VfRow {
+  unsigned long long sum;  // Z; at temperature 0 the maximum's key and, below it, ~its index; 0: no distribution
   uint32_t top;            // order key of the largest logit, 0: none
-  uint32_t best;           // temperature 0: ~index of the first maximum, 0: none
+  uint32_t arrived;        // (a sequence's first row) slices done
   float logit, q;          // of the drafted token
-  int drafted;             // there is one, inside the vocabulary
-  uint32_t arrived;        // (a sequence's first row) slices weighed
+  int drafted, pad;        // there is one, inside the vocabulary
 };
+// (past L1: other CTAs' atomics, and neighbours in a line)
+__device__ __forceinline__ VfRow vf_row(const VfRow* r) {
+  VfRow x;
+  reinterpret_cast<uint4*>(&x)[0] = __ldcg(reinterpret_cast<const uint4*>(r));
+  reinterpret_cast<uint4*>(&x)[1] = __ldcg(reinterpret_cast<const uint4*>(r) + 1);
+  return x;
+}
 
 struct VfArgs {
   const void* logits;
@@ -214,22 +221,6 @@ __global__ void __launch_bounds__(kVfThreads) k_verify_sum(VfArgs a) {
   const VfVec<E> vec((const E*)a.logits + (int64_t)blockIdx.y * a.row_stride, a.V);
   const float best = vf_unkey(row->top);
   const int j0 = blockIdx.x * kVfThreads * a.per + threadIdx.x;
-  if (a.inv_temp == 0.f) {
-    if (best == -INFINITY) return;
-    uint32_t at = 0xffffffffu;
-    for (int k = 0; k < a.per; ++k) {
-      const int j = j0 + k * kVfThreads;
-      if (j >= vec.count) break;
-      float x[N];
-      vec.unpack(vec.load(j), x);
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (x[e] == best) at = min(at, (uint32_t)(vec.first(j) + e));
-    }
-    at = __reduce_min_sync(0xffffffffu, at);
-    if ((threadIdx.x & 31) == 0 && at != 0xffffffffu) atomicMax(&row->best, ~at);
-    return;
-  }
   // rounding is monotonic: the largest product is the largest logit's
   const float mx = __fmul_rn(best, a.inv_temp);
   if (!(fabsf(mx) < INFINITY)) return;
@@ -248,7 +239,7 @@ __global__ void __launch_bounds__(kVfThreads) k_verify_sum(VfArgs a) {
 
 // What a sequence's rows say: drafts accepted, and the row the next token is drawn from.
 struct VfSeq {
-  const VfRow* row;
+  VfRow row;
   int accepted;
   bool refused;
 };
@@ -259,12 +250,12 @@ __device__ __forceinline__ VfSeq vf_decide(const VfArgs& a, int b, float* prob) 
   bool ok = false;
   *prob = 0.f;
   if (lane < nd) {
-    const VfRow r = rows[lane];
-    if (r.drafted) {
-      if (a.inv_temp == 0.f) {
-        ok = r.best != 0 && (int)~r.best == a.ids[(int64_t)b * a.T + lane];
-        *prob = ok ? 1.f : 0.f;
-      } else {
+    const VfRow r = vf_row(rows + lane);
+    if (a.inv_temp == 0.f) {
+      ok = r.sum != 0 && (int)~(uint32_t)r.sum == a.ids[(int64_t)b * a.T + lane];
+      *prob = ok ? 1.f : 0.f;
+    } else if (r.drafted) {
+      {
         VfFix f;
         const float w = f.add(vf_exp(r.logit, a.inv_temp, __fmul_rn(vf_unkey(r.top), a.inv_temp)));
         const float p = r.sum ? __fdiv_rn(w, (float)r.sum * 0x1p-40f) : 0.f;
@@ -276,7 +267,7 @@ __device__ __forceinline__ VfSeq vf_decide(const VfArgs& a, int b, float* prob) 
   VfSeq s;
   s.accepted = __ffs((int)__ballot_sync(0xffffffffu, !ok)) - 1;  // nd <= 31: lane nd has none
   s.refused = s.accepted < nd;
-  s.row = rows + s.accepted;
+  s.row = vf_row(rows + s.accepted);
   return s;
 }
 
@@ -295,9 +286,9 @@ struct VfDraw {
     id = s.refused ? a.ids[(int64_t)b * a.T + s.accepted] : -1;
     q = s.refused && a.probs ? a.probs + ((int64_t)b * a.T + s.accepted) * a.V : nullptr;
     q_vec = ((reinterpret_cast<uintptr_t>(q) - vec.skew * 4) & 15u) == 0;
-    z = (float)s.row->sum * 0x1p-40f;
+    z = (float)s.row.sum * 0x1p-40f;
     inv_temp = a.inv_temp;
-    mx = __fmul_rn(vf_unkey(s.row->top), a.inv_temp);
+    mx = __fmul_rn(vf_unkey(s.row.top), a.inv_temp);
   }
   // adds the weights of vector j to f; `each`: the running sums after every element
   __device__ __forceinline__ void weigh(int j, VfFix& f, unsigned long long* each) const {
@@ -363,9 +354,9 @@ __device__ __forceinline__ void vf_pick(const VfArgs& a, int b, const VfSeq& s, 
   if (tid < T) a.accept_prob[(int64_t)b * T + tid] = prob;
   if (tid == 0) {
     a.accepted[b] = s.accepted;
-    token = a.inv_temp == 0.f && s.row->best != 0 ? (int)~s.row->best : -1;
+    token = a.inv_temp == 0.f && s.row.sum != 0 ? (int)~(uint32_t)s.row.sum : -1;
   }
-  if (a.inv_temp != 0.f && s.row->sum != 0) {
+  if (a.inv_temp != 0.f && s.row.sum != 0) {
     VfDraw<E> draw(a, b, s);
     constexpr int N = VfDraw<E>::N;
     unsigned long long* steps = a.steps + (int64_t)b * a.step_stride;
@@ -445,7 +436,7 @@ __global__ void __launch_bounds__(kVfThreads) k_verify_weigh(VfArgs a) {
   const float u = a.u[(int64_t)b * (a.T + 1) + a.T];
   float prob;
   const VfSeq s = vf_decide(a, b, &prob);
-  if (s.row->sum != 0) {
+  if (s.row.sum != 0) {
     const VfDraw<E> draw(a, b, s);
     for (int k = 0; k < a.per; ++k) {
       const int step = (blockIdx.x * a.per + k) * kVfWarps + warp, j = step * 32 + lane;
@@ -465,13 +456,62 @@ __global__ void __launch_bounds__(kVfThreads) k_verify_weigh(VfArgs a) {
   vf_pick<E>(a, b, s, prob, u);
 }
 
-// temperature 0: nothing to weigh
+// Temperature 0, one launch: grid (slices, rows); slices meet in the maximum of (key, ~index),
+// and the last CTA of a sequence to arrive decides.
 template <typename E>
 __global__ void __launch_bounds__(kVfThreads) k_verify_greedy(VfArgs a) {
+  __shared__ bool last;
   pdl_wait();
+  const int b = blockIdx.y / (a.T + 1), i = blockIdx.y % (a.T + 1), nd = vf_drafts(a, b);
+  if (i > nd) return;
+  constexpr int N = VfVec<E>::N;
+  const VfVec<E> vec((const E*)a.logits + (int64_t)blockIdx.y * a.row_stride, a.V);
+  float best = -INFINITY;
+  int at = 0;
+  const int j0 = blockIdx.x * kVfThreads * a.per + threadIdx.x;
+  const uint32_t low = sizeof(E) == 2 ? 0xff80ff80u : 0xff800000u;
+  for (int k = 0; k < a.per; k += 4) {  // four loads in flight
+    uint4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = j0 + (k + u) * kVfThreads;
+      v[u] = k + u < a.per && j < vec.count ? vec.load(j) : make_uint4(low, low, low, low);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float was = best;
+      best = vec.max(v[u], best);
+      if (best > was) {  // a new maximum: its first index in this vector
+        float x[N];
+        vec.unpack(v[u], x);
+        at = vec.first(j0 + (k + u) * kVfThreads);
+        int e = 0;
+#pragma unroll
+        for (int y = N - 1; y >= 0; --y)
+          if (x[y] == best) e = y;
+        at += e;
+      }
+    }
+  }
+  // (-0 as +0: they are equal, the first of them counts)
+  unsigned long long key = best > -INFINITY ? (unsigned long long)vf_key(best + 0.f) << 32 | (uint32_t)~at : 0ull;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const unsigned long long y = __shfl_xor_sync(0xffffffffu, key, o);
+    key = y > key ? y : key;
+  }
+  if ((threadIdx.x & 31) == 0) {
+    if (key) atomicMax(&a.rows[blockIdx.y].sum, key);
+    __threadfence();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(&a.rows[(int64_t)b * (a.T + 1)].arrived, 1u) == gridDim.x * (nd + 1) - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
   float prob;
-  const VfSeq s = vf_decide(a, blockIdx.x, &prob);
-  vf_pick<E>(a, blockIdx.x, s, prob, 0.f);
+  const VfSeq s = vf_decide(a, b, &prob);
+  vf_pick<E>(a, b, s, prob, 0.f);
 }
 
 template <typename E>
@@ -486,14 +526,15 @@ static int verify_launch(VfArgs& a, int B, cudaStream_t s) {
     return (unsigned)((most + kVfThreads * a.per - 1) / (kVfThreads * a.per));
   };
   const unsigned slices = cut(B * (a.T + 1));
-  JSX_CUDA(launch_kernel(k_verify_max<E>, dim3(slices, B * (a.T + 1)), dim3(kVfThreads), 0, s, a));
-  JSX_CUDA(launch_kernel(k_verify_sum<E>, dim3(slices, B * (a.T + 1)), dim3(kVfThreads), 0, s, a));
-  if (a.inv_temp != 0.f) {
-    const unsigned n = cut(B);
-    JSX_CUDA(launch_kernel(k_verify_weigh<E>, dim3(n, B), dim3(kVfThreads), 0, s, a));
-  } else {
-    JSX_CUDA(launch_kernel(k_verify_greedy<E>, dim3(B), dim3(kVfThreads), 0, s, a));
+  const dim3 grid(slices, B * (a.T + 1));
+  if (a.inv_temp == 0.f) {
+    JSX_CUDA(launch_kernel(k_verify_greedy<E>, grid, dim3(kVfThreads), 0, s, a));
+    return JSX_OK;
   }
+  JSX_CUDA(launch_kernel(k_verify_max<E>, grid, dim3(kVfThreads), 0, s, a));
+  JSX_CUDA(launch_kernel(k_verify_sum<E>, grid, dim3(kVfThreads), 0, s, a));
+  const unsigned n = cut(B);
+  JSX_CUDA(launch_kernel(k_verify_weigh<E>, dim3(n, B), dim3(kVfThreads), 0, s, a));
   return JSX_OK;
 }
 

@@ -154,6 +154,24 @@ def test_one_workspace_for_calls_of_several_shapes(jsx, cuda):
             assert not shared.any()
 
 
+@pytest.mark.parametrize("f32", [False, True])
+def test_greedy_takes_the_first_of_equals(jsx, cuda, f32):
+    """Equal maxima in one vector, in several and in several slices; +0 and -0 are equal."""
+    V = 40000
+    x = torch.full((4, 2, V), -1.0, device="cuda", dtype=torch.float32 if f32 else torch.bfloat16)
+    x[0, :, [9001, 9002, 30000]] = 2.0
+    x[1, :, 17], x[1, :, 39999] = -0.0, 0.0
+    x[2, :, 39998], x[2, :, 23] = -0.0, 0.0
+    x[3] = float("nan")
+    x[3, :, 5], x[3, :, 20000] = float("inf"), float("inf")
+    want = torch.tensor([9001, 17, 23, 5], dtype=torch.int32, device="cuda")
+    ws = jsx.kernels.verify_workspace(4, 1, V, x.device)
+    acc, tok, pr = jsx.kernels.verify_drafts(x, want.view(4, 1), None, ws, temperature=0.0)
+    assert (acc == 1).all() and (pr == 1).all() and torch.equal(tok, want.view(4, 1).expand(4, 2))
+    acc, tok, pr = jsx.kernels.verify_drafts(x, (want + 1).view(4, 1), None, ws, temperature=0.0)
+    assert (acc == 0).all() and (pr == 0).all() and torch.equal(tok[:, 0], want) and (tok[:, 1] == -1).all()
+
+
 def test_refusals(jsx, cuda):
     K = jsx.kernels
     x = torch.zeros(2, 3, 100, device="cuda")
