@@ -66,7 +66,7 @@ struct VfArgs {
   const int32_t* n_draft;
   const float* u;  // [B][T + 1]
   VfRow* rows;     // [B][T + 1]
-  unsigned long long* steps;  // [B][step_stride]
+  unsigned long long* steps;  // [B][T + 1][step_stride] sums of 32 vectors each (with q: a sequence's first row only)
   int32_t* accepted;
   int32_t* tokens;
   float* accept_prob;
@@ -211,32 +211,6 @@ __global__ void __launch_bounds__(kVfThreads) k_verify_max(VfArgs a) {
   }
 }
 
-template <typename E>
-__global__ void __launch_bounds__(kVfThreads) k_verify_sum(VfArgs a) {
-  pdl_wait();
-  const int b = blockIdx.y / (a.T + 1), i = blockIdx.y % (a.T + 1);
-  if (i > vf_drafts(a, b)) return;
-  constexpr int N = VfVec<E>::N;
-  VfRow* row = a.rows + blockIdx.y;
-  const VfVec<E> vec((const E*)a.logits + (int64_t)blockIdx.y * a.row_stride, a.V);
-  const float best = vf_unkey(row->top);
-  const int j0 = blockIdx.x * kVfThreads * a.per + threadIdx.x;
-  // rounding is monotonic: the largest product is the largest logit's
-  const float mx = __fmul_rn(best, a.inv_temp);
-  if (!(fabsf(mx) < INFINITY)) return;
-  VfFix f;
-  for (int k = 0; k < a.per; ++k) {
-    const int j = j0 + k * kVfThreads;
-    if (j >= vec.count) break;
-    float x[N];
-    vec.unpack(vec.load(j), x);
-#pragma unroll
-    for (int e = 0; e < N; ++e) f.add(vf_exp(x[e], a.inv_temp, mx));
-  }
-  const unsigned long long s = f.warp_sum();
-  if ((threadIdx.x & 31) == 0 && s) atomicAdd(&row->sum, s);
-}
-
 // What a sequence's rows say: drafts accepted, and the row the next token is drawn from.
 struct VfSeq {
   VfRow row;
@@ -346,8 +320,9 @@ __device__ __forceinline__ unsigned long long vf_scan(unsigned long long x) {  /
 }
 
 // By one CTA per sequence: the draw, the outputs, and the workspace zero again.
+// steps: of the row that is drawn from; without q they are the row's own weights.
 template <typename E>
-__device__ __forceinline__ void vf_pick(const VfArgs& a, int b, const VfSeq& s, float prob, float u) {
+__device__ __forceinline__ void vf_pick(const VfArgs& a, int b, const VfSeq& s, float prob, float u, unsigned long long* steps) {
   __shared__ unsigned long long warps[kVfWarps], reached;
   __shared__ int token;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, T = a.T;
@@ -359,9 +334,16 @@ __device__ __forceinline__ void vf_pick(const VfArgs& a, int b, const VfSeq& s, 
   if (a.inv_temp != 0.f && s.row.sum != 0) {
     VfDraw<E> draw(a, b, s);
     constexpr int N = VfDraw<E>::N;
-    unsigned long long* steps = a.steps + (int64_t)b * a.step_stride;
     const int n = (draw.vec.count + 31) / 32, per = (n + kVfThreads - 1) / kVfThreads;
     unsigned long long mine, before, total;
+    if (!a.probs && s.refused && s.row.drafted) {  // without the refused token
+      if (tid == 0) {
+        VfFix f;
+        f.add(vf_exp(s.row.logit, a.inv_temp, draw.mx));
+        steps[(draw.id + draw.vec.skew) / N / 32] -= f.sum();
+      }
+      __syncthreads();
+    }
     for (;;) {
       // thread t has steps [t per, (t + 1) per)
       mine = 0;
@@ -392,7 +374,7 @@ __device__ __forceinline__ void vf_pick(const VfArgs& a, int b, const VfSeq& s, 
     const unsigned long long at = vf_threshold(total, u);
     if (before <= at && at < before + mine) {  // one thread: its step with the crossing
       int k = tid * per;
-      for (unsigned long long x; before + (x = steps[k]) <= at; ++k) before += x;
+      for (unsigned long long x; before + (x = __ldcg(steps + k)) <= at; ++k) before += x;
       reached = before;
       token = k;
     }
@@ -414,7 +396,6 @@ __device__ __forceinline__ void vf_pick(const VfArgs& a, int b, const VfSeq& s, 
         token = draw.vec.first(j) + e;
       }
     }
-    for (int k = tid; k < n; k += kVfThreads) steps[k] = 0;  // (the next call's records may lie here)
   }
   __syncthreads();
   if (tid <= T) {
@@ -424,10 +405,64 @@ __device__ __forceinline__ void vf_pick(const VfArgs& a, int b, const VfSeq& s, 
     a.tokens[(int64_t)b * (T + 1) + tid] = t;
     a.rows[(int64_t)b * (T + 1) + tid] = VfRow{};
   }
+  if (a.inv_temp != 0.f) {  // (the next call's records may lie here)
+    const int64_t n = (int64_t)a.step_stride * (a.probs ? 1 : T + 1);
+    for (int64_t k = tid; k < n; k += kVfThreads) a.steps[(int64_t)b * (T + 1) * a.step_stride + k] = 0;
+  }
 }
 
-// grid (slices, sequences): the weights' sums of every step (32 vectors, a warp); the last
-// CTA of a sequence to arrive draws its token
+// grid as above: the rows' sums.  Without draft distributions (kDraw) also the sums of every
+// step (32 vectors, a warp), which are all that a draw needs: the last CTA of a sequence to
+// arrive draws its token.
+template <typename E, bool kDraw>
+__global__ void __launch_bounds__(kVfThreads) k_verify_sum(VfArgs a) {
+  pdl_wait();
+  const int b = blockIdx.y / (a.T + 1), i = blockIdx.y % (a.T + 1), nd = vf_drafts(a, b);
+  if (i > nd) return;
+  constexpr int N = VfVec<E>::N;
+  VfRow* row = a.rows + blockIdx.y;
+  const VfVec<E> vec((const E*)a.logits + (int64_t)blockIdx.y * a.row_stride, a.V);
+  // rounding is monotonic: the largest product is the largest logit's
+  const float mx = __fmul_rn(vf_unkey(row->top), a.inv_temp);
+  const int lane = threadIdx.x & 31, first = blockIdx.x * kVfThreads * a.per;
+  if (fabsf(mx) < INFINITY) {
+    VfFix f;
+    unsigned long long sum = 0;
+    for (int k = 0; k < a.per; ++k) {
+      const int j = first + k * kVfThreads + (int)threadIdx.x;
+      if (j - lane >= vec.count) break;
+      if (j < vec.count) {
+        float x[N];
+        vec.unpack(vec.load(j), x);
+#pragma unroll
+        for (int e = 0; e < N; ++e) f.add(vf_exp(x[e], a.inv_temp, mx));
+      }
+      if (kDraw) {
+        const unsigned long long y = f.warp_sum();
+        if (lane == 0) a.steps[(int64_t)blockIdx.y * a.step_stride + j / 32] = y;
+        sum += y;
+        f = VfFix();
+      }
+    }
+    if (!kDraw) sum = f.warp_sum();
+    if (lane == 0 && sum) atomicAdd(&row->sum, sum);
+  }
+  if (!kDraw) return;
+  __shared__ bool last;
+  if (lane == 0) __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(&a.rows[(int64_t)b * (a.T + 1)].arrived, 1u) == gridDim.x * (nd + 1) - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  float prob;
+  const VfSeq s = vf_decide(a, b, &prob);
+  vf_pick<E>(a, b, s, prob, a.u[(int64_t)b * (a.T + 1) + a.T],
+             a.steps + ((int64_t)b * (a.T + 1) + s.accepted) * a.step_stride);
+}
+
+// grid (slices, sequences), with draft distributions: the weights' sums of every step of the
+// row that a token is drawn from; the last CTA of a sequence to arrive draws it
 template <typename E>
 __global__ void __launch_bounds__(kVfThreads) k_verify_weigh(VfArgs a) {
   __shared__ bool last;
@@ -436,6 +471,7 @@ __global__ void __launch_bounds__(kVfThreads) k_verify_weigh(VfArgs a) {
   const float u = a.u[(int64_t)b * (a.T + 1) + a.T];
   float prob;
   const VfSeq s = vf_decide(a, b, &prob);
+  unsigned long long* steps = a.steps + (int64_t)b * (a.T + 1) * a.step_stride;
   if (s.row.sum != 0) {
     const VfDraw<E> draw(a, b, s);
     for (int k = 0; k < a.per; ++k) {
@@ -444,7 +480,7 @@ __global__ void __launch_bounds__(kVfThreads) k_verify_weigh(VfArgs a) {
       VfFix f;
       if (j < draw.vec.count) draw.weigh(j, f, nullptr);
       const unsigned long long x = f.warp_sum();
-      if (lane == 0) a.steps[(int64_t)b * a.step_stride + step] = x;
+      if (lane == 0) steps[step] = x;
     }
   }
   if (lane == 0) __threadfence();
@@ -453,7 +489,7 @@ __global__ void __launch_bounds__(kVfThreads) k_verify_weigh(VfArgs a) {
   __syncthreads();
   if (!last) return;
   __threadfence();
-  vf_pick<E>(a, b, s, prob, u);
+  vf_pick<E>(a, b, s, prob, u, steps);
 }
 
 // Temperature 0, one launch: grid (slices, rows); slices meet in the maximum of (key, ~index),
@@ -511,7 +547,7 @@ __global__ void __launch_bounds__(kVfThreads) k_verify_greedy(VfArgs a) {
   __threadfence();
   float prob;
   const VfSeq s = vf_decide(a, b, &prob);
-  vf_pick<E>(a, b, s, prob, 0.f);
+  vf_pick<E>(a, b, s, prob, 0.f, nullptr);
 }
 
 template <typename E>
@@ -532,7 +568,11 @@ static int verify_launch(VfArgs& a, int B, cudaStream_t s) {
     return JSX_OK;
   }
   JSX_CUDA(launch_kernel(k_verify_max<E>, grid, dim3(kVfThreads), 0, s, a));
-  JSX_CUDA(launch_kernel(k_verify_sum<E>, grid, dim3(kVfThreads), 0, s, a));
+  if (!a.probs) {
+    JSX_CUDA(launch_kernel(k_verify_sum<E, true>, grid, dim3(kVfThreads), 0, s, a));
+    return JSX_OK;
+  }
+  JSX_CUDA(launch_kernel(k_verify_sum<E, false>, grid, dim3(kVfThreads), 0, s, a));
   const unsigned n = cut(B);
   JSX_CUDA(launch_kernel(k_verify_weigh<E>, dim3(n, B), dim3(kVfThreads), 0, s, a));
   return JSX_OK;
@@ -547,7 +587,7 @@ static int64_t vf_steps(int V) { return (V + 6) / 4 / 32 + 1; }
 
 extern "C" int jsx_verify_workspace_size(int B, int T, int V, size_t* bytes) {
   JSX_REQUIRE(bytes && B >= 1 && T >= 0 && T <= kVfMaxDraft && V >= 1 && V <= kVfMaxVocab, "bad arguments");
-  *bytes = (size_t)B * (T + 1) * sizeof(VfRow) + (size_t)B * vf_steps(V) * 8;
+  *bytes = (size_t)B * (T + 1) * sizeof(VfRow) + (size_t)B * (T + 1) * vf_steps(V) * 8;
   return JSX_OK;
 }
 
