@@ -16,18 +16,20 @@
 // running sum exceeds floor(u total), u taken to 24 bits.  The floor costs a row
 // at most V 2^-41 of its mass (7e-8 at 151552 tokens).
 //
-// Three launches over slices of rows: the rows' maxima, their sums, and the weights of the
-// one row per sequence that a token is drawn from, summed per step of 32 vectors; the last
-// CTA of a sequence finds the step with the crossing and weighs it again.  Slices meet in
-// integer atomics (maximum, sum), so they need no order and no wait; the second pass
-// over the logits comes from L2 (at most 126 MB of it).  At temperature 0 (greedy: p is
-// 1 at the lowest index of the maximum) nothing is weighed, and one launch does it all.
+// Launches over slices of rows.  With draft distributions three: the rows' maxima, their sums,
+// and the weights of the one row per sequence that a token is drawn from, summed per step of 32
+// vectors.  Without, the second launch keeps the sums of its steps, which are those weights'.  At
+// temperature 0 (greedy: p is 1 at the lowest index of the maximum) one launch finds the maxima
+// with their indexes.  The last CTA of a sequence to arrive decides, finds the step with the
+// crossing and weighs it again.  Slices meet in integer atomics (maximum, sum), so they need no
+// order and no wait; the second pass over the logits comes from L2 (at most 126 MB of it).
 // Bound: from some 20 rows on the exponentials' instructions (18 per logit with the exact
 // sum, 75% of the issue slots) rather than the bytes; launches below.  32 x 5 rows of 151552
-// with draft distributions: 44 us, 12 of them the maxima (4.0 TB/s) and 21 the sums; 1 x 5:
-// 13.5 us; 16 x 8 rows of 32003, greedy: 5.8 us (7.9 in three launches, which also cost the
-// host 5 us more).  One cluster per row with distributed
-// shared memory instead of atomics: 79 us.
+// with draft distributions: 44 us, 12 of them the maxima (4.0 TB/s) and 21 the sums; 1 x 5
+// without: 13.0 us; 16 x 8 rows of 32003, greedy: 5.8 us (7.9 in three launches, which also
+// cost the host 5 us more).  One cluster per row with distributed shared memory instead of
+// atomics: 79 us; one cooperative launch in which the slices wait for one another: 17.7 against
+// 13.5 us at 1 x 5.
 // NaN logits and a row's -inf entries have no mass; a row with no mass at all, or
 // with +inf, accepts nothing and draws token -1 (greedy takes +inf as the maximum).
 #include <math.h>
