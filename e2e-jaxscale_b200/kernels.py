@@ -54,8 +54,8 @@ def pdl_enabled() -> bool:
 
 def device_error() -> int:
     """jsx_device_error: JSX_ETIMEDOUT (3) when a bounded wait of the whole-step kernel,
-    the streaming GEMV or the tensor-core projections gave up since the last call,
-    else 0 (reads and clears the error words; synchronous)."""
+    the streaming GEMV, the tensor-core projections or the attention over 4-bit pages gave up
+    since the last call, else 0 (reads and clears the error words; synchronous)."""
     out = ctypes.c_int(0)
     call("jsx_device_error", ctypes.byref(out))
     return out.value
