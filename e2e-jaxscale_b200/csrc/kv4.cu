@@ -3,7 +3,9 @@
 // Append, per 16 values x of a row: s = e4m3(min(max |x| / 6, 448)), code =
 // e2m1(x / s) (0 where s is 0), both rounded to nearest even.  A bf16 value has
 // 8 significant bits and a scale 4, so a quotient is either exactly on a code's
-// rounding boundary or at least 2^-10 from it; x (1/s) is within 2^-21 of x / s.
+// rounding boundary or at least 2^-10 from it; x (1/s) is within 2^-21 of x / s, 1/s within
+// 2^-22.  The scale too comes from a product, max |x| (1/6): over all 32640 bf16 magnitudes it
+// rounds to the same e4m3 as the quotient.
 // Rounding it to multiples of 2^-13 (one fused multiply-add against 1536 and a
 // subtraction) therefore gives the codes of the exact quotient, without 16
 // divisions per group.  The largest magnitude is an integer maximum over the
@@ -11,13 +13,14 @@
 // scale and reads back as NaN; infinities saturate at 6 x 448.
 //
 // Both kernels move 32 bytes of bf16 per 9 bytes of page.  One thread handles a group
-// of a K row and the same of its V row: two 16-byte accesses each on the bf16 side, 8
-// bytes of codes and one scale byte on the page side; the threads of a row are adjacent.
+// of a K row and the same of its V row: two 16-byte accesses each on the bf16 side (dealt to
+// pairs of lanes, kv4_swap), 8 bytes of codes and one scale byte on the page side; the threads of a row are adjacent.
 // (8 values a thread would make every access whole, but doubles the index arithmetic:
 // 30 against 23 us for 32 x 1024 rows of 2 heads there and back.)
 //
-// Bound: memory for many rows (32 x 1024 rows of 2 heads there and back: 21.6 us, 86 MB of
-// rows and pages, 4.0 TB/s, much of it in L2), the launch for few (32 x 1: 3.1 us on the device).
+// Bound: memory for many rows (32 x 1024 rows of 2 heads there and back: 18.0 us, 86 MB of
+// rows and pages, 4.8 TB/s, much of it in L2; 21.6 us while a lane's accesses were 16 bytes of
+// every 32), the launch for few (32 x 1: 3.1 us on the device).
 #include "common.cuh"
 #include "kv4.cuh"
 #include "launch.cuh"
@@ -71,6 +74,21 @@ __device__ __forceinline__ Kv4Unit kv4_unit(const Kv4RowArgs& a, int b, uint32_t
   return x;
 }
 
+// Two lanes access 32 bytes side by side, the even one's group and then the odd one's, so that
+// every access is of whole 32-byte sectors; this takes them to the lanes' own groups and back.
+// (A row has an even number of groups: both lanes have one or neither.)
+__device__ __forceinline__ void kv4_swap(uint4& lo, uint4& hi, bool odd) {
+  uint32_t x[4] = {lo.x, lo.y, lo.z, lo.w}, y[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t z = __shfl_xor_sync(3u << (threadIdx.x & 30), odd ? x[i] : y[i], 1);
+    x[i] = odd ? z : x[i];
+    y[i] = odd ? y[i] : z;
+  }
+  lo = make_uint4(x[0], x[1], x[2], x[3]);
+  hi = make_uint4(y[0], y[1], y[2], y[3]);
+}
+
 template <int D>
 __global__ void __launch_bounds__(kKv4Threads) k_kv4_append(Kv4RowArgs a) {
   pdl_wait();
@@ -78,14 +96,17 @@ __global__ void __launch_bounds__(kKv4Threads) k_kv4_append(Kv4RowArgs a) {
   for (uint32_t u = blockIdx.x * kKv4Threads + threadIdx.x; u < a.units; u += gridDim.x * kKv4Threads) {
     const Kv4Unit x = kv4_unit<D>(a, b, u, first, used);
     if (!x.inside) continue;
+    const bool odd = threadIdx.x & 1;
     uint4 p[2][2];  // in flight together with the page number
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const bf16* row = (k ? a.v : a.k) + x.row;
+      const bf16* row = (k ? a.v : a.k) + x.row - (odd ? 8 : 0);
       p[k][0] = *reinterpret_cast<const uint4*>(row);
-      p[k][1] = *reinterpret_cast<const uint4*>(row + 8);
+      p[k][1] = *reinterpret_cast<const uint4*>(row + 16);
     }
     if (!x.paged) continue;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) kv4_swap(p[k][0], p[k][1], odd);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const uint32_t w[8] = {p[k][0].x, p[k][0].y, p[k][0].z, p[k][0].w, p[k][1].x, p[k][1].y, p[k][1].z, p[k][1].w};
@@ -93,9 +114,9 @@ __global__ void __launch_bounds__(kKv4Threads) k_kv4_append(Kv4RowArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) mx = __vmaxu2(mx, w[i] & 0x7fff7fffu);
       const float top = __uint_as_float(max(mx & 0xffffu, mx >> 16) << 16);
-      const uint32_t sc = f32_to_e4m3(__fdiv_rn(top, 6.f));
+      const uint32_t sc = f32_to_e4m3(top * (1.f / 6.f));
       const float s = __half2float(__ushort_as_half((unsigned short)(e4m3x2_to_h2(sc) & 0xffffu)));
-      const float inv = s == 0.f ? 0.f : __frcp_rn(s);
+      const float inv = s == 0.f ? 0.f : __fdividef(1.f, s);
       float q[2][8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -136,9 +157,12 @@ __global__ void __launch_bounds__(kKv4Threads) k_kv4_read(Kv4RowArgs a) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&y));
         o[i] = pack2(f.x, f.y);
       }
-      bf16* row = (k ? a.v : a.k) + x.row;
-      *reinterpret_cast<uint4*>(row) = make_uint4(o[0], o[1], o[2], o[3]);
-      *reinterpret_cast<uint4*>(row + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+      const bool odd = threadIdx.x & 1;
+      uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+      kv4_swap(lo, hi, odd);
+      bf16* row = (k ? a.v : a.k) + x.row - (odd ? 8 : 0);
+      *reinterpret_cast<uint4*>(row) = lo;
+      *reinterpret_cast<uint4*>(row + 16) = hi;
     }
   }
 }
