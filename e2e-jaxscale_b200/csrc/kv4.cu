@@ -12,11 +12,11 @@
 // bf16 bit patterns, where NaN is above infinity: a group with a NaN gets a NaN
 // scale and reads back as NaN; infinities saturate at 6 x 448.
 //
-// Both kernels move 32 bytes of bf16 per 9 bytes of page.  One thread handles a group
-// of a K row and the same of its V row: two 16-byte accesses each on the bf16 side (dealt to
-// pairs of lanes, kv4_swap), 8 bytes of codes and one scale byte on the page side; the threads of a row are adjacent.
-// (8 values a thread would make every access whole, but doubles the index arithmetic:
-// 30 against 23 us for 32 x 1024 rows of 2 heads there and back.)
+// Both kernels move 32 bytes of bf16 per 9 bytes of page.  One thread handles a group of a K row
+// and the same of its V row: two 16-byte accesses each on the bf16 side (dealt to pairs of
+// lanes, kv4_swap), 8 bytes of codes and one scale byte on the page side; the threads of a row
+// are adjacent.  (8 values a thread would make every access whole, but doubles the index
+// arithmetic: 30 against 23 us for 32 x 1024 rows of 2 heads there and back.)
 //
 // Bound: memory for many rows (32 x 1024 rows of 2 heads there and back: 18.0 us, 86 MB of
 // rows and pages, 4.8 TB/s, much of it in L2; 21.6 us while a lane's accesses were 16 bytes of
