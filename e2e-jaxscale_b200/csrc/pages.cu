@@ -161,7 +161,9 @@ struct PgResizeArgs {
   int S, slots, P, pt;
 };
 
-// Slots of sequence s: in use before, in use after, and the first that will be written.
+// Slots of sequence s: in use before, in use after, and the first that will be written.  A row
+// keeps no more than its pages hold, so first <= before: the slots from `before` on that are
+// counted as taken are the ones that are assigned, and no entry of the list is left unwritten.
 struct PgRow {
   int before, after, first, over;  // over: pages beyond the table's slots
   int keep;
@@ -169,9 +171,9 @@ struct PgRow {
 __device__ __forceinline__ PgRow pg_row(const PgResizeArgs& a, int s) {
   PgRow r;
   const int need = max(a.need[s], 0);
-  r.keep = min(max(a.keep[s], 0), need);
   const int n = need / a.pt + (need % a.pt != 0);
   r.before = pg_held(a.held, s, a.slots);
+  r.keep = (int)min((long long)min(max(a.keep[s], 0), need), (long long)r.before * a.pt);
   r.after = min(n, a.slots);
   r.over = min(n - r.after, 1 << 15);  // (a sum over 2^15 rows stays in 31 bits)
   r.first = r.keep / a.pt;

@@ -641,8 +641,8 @@ def pages_fork(table, held, refs, parent, table_out=None, held_out=None, refs_ou
 
 
 def pages_resize(table, held, refs, keep, need, pool, page_tokens, workspace, missing=None):
-    """In place: row b keeps its first keep[b] tokens and has pages of its own for need[b]
-    (include/jsx.h jsx_pages_resize).  Returns missing, int32 [1] on the device: 0, or how many
+    """In place: row b keeps its first keep[b] tokens (no more than its pages hold) and has pages
+    of its own from there up to need[b] (include/jsx.h jsx_pages_resize).  Returns missing, int32 [1] on the device: 0, or how many
     pages there were too few (nothing is changed then)."""
     S, slots, P_ = _pages(table, held, refs)
     _need(keep, "keep", I32)

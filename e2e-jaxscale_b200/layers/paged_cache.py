@@ -36,8 +36,8 @@ class PagedKV4Cache:
 
     # ---- pages ----
     def reserve(self, keep: torch.Tensor, need: torch.Tensor) -> torch.Tensor:
-        """Every sequence keeps its first keep[b] tokens and gets pages of its own for tokens
-        keep[b] .. need[b] - 1; the rest goes back.  Returns `missing` (int32 [1] on the device):
+        """Every sequence keeps its first keep[b] tokens (no more than its pages hold) and gets pages
+        of its own from there to token need[b] - 1; the rest goes back.  Returns `missing` (int32 [1] on the device):
         0, or how many pages there were too few; nothing is changed then."""
         return K.pages_resize(self.table, self.held, self.refs, keep, need, self.pool, self.page_tokens, self._ws,
                               missing=self.missing)

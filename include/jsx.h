@@ -470,13 +470,15 @@ int jsx_pages_workspace_size(int sequences, int slots, int num_pages, size_t* by
 int jsx_pages_fork(const int32_t* table, const int32_t* held, const int32_t* refs,
                    const int32_t* parent, int32_t* table_out, int32_t* held_out, int32_t* refs_out,
                    int sequences, int slots, int num_pages, void* stream);
-/* Row b keeps its first keep[b] tokens (at most need[b]) and gets pages for need[b]
- * tokens.  Pages from keep[b] on that others hold too are replaced by free ones
- * (their bytes are copied in every layer of pool [layers][num_pages][page_bytes] if
- * they hold kept tokens); pages beyond need[b] are given back.  Free pages are taken
- * lowest first, in sequence and slot order, from those that were free before the
- * call.  *missing = 0, or, with nothing changed, how many pages there were too few
- * (free ones or table slots). */
+/* Row b keeps its first keep[b] tokens (at most need[b], and at most what its held[b]
+ * pages have room for) and gets pages for need[b] tokens: every slot from there to the
+ * last that need[b] uses has one.  Pages from token keep[b] on that others hold too are
+ * replaced by free ones; their bytes are copied in every layer of pool
+ * [layers][num_pages][page_bytes] if they hold kept tokens.  (So is the page that keep[b]
+ * ends inside, also when need[b] is keep[b].)  Pages beyond need[b] are given back.  Free
+ * pages are taken lowest first, in sequence and slot order, from those that were free
+ * before the call.  *missing = 0, or, with nothing changed, how many pages there were too
+ * few (free ones or table slots). */
 int jsx_pages_resize(int32_t* table, int32_t* held, int32_t* refs, const int32_t* keep,
                      const int32_t* need, void* pool, int layers, size_t page_bytes, int sequences,
                      int slots, int num_pages, int page_tokens, int32_t* missing, void* workspace,

@@ -124,7 +124,7 @@ def pages_resize(table, held, refs, keep, need, page_tokens):
     give_back = []
     for b in range(S):
         nd = max(int(need[b]), 0)
-        kp = min(max(int(keep[b]), 0), nd)
+        kp = min(max(int(keep[b]), 0), nd, int(h[b]) * page_tokens)
         n = -(-nd // page_tokens)
         over += max(n - slots, 0)
         n = min(n, slots)
