@@ -32,6 +32,8 @@
 // 13.5 us at 1 x 5.
 // NaN logits and a row's -inf entries have no mass; a row with no mass at all, or
 // with +inf, accepts nothing and draws token -1 (greedy takes +inf as the maximum).
+// A finite maximum whose quotient by the temperature overflows (a row whose mask left only the
+// type's lowest value, say) leaves the mass to the entries equal to it: see vf_inv.
 #include <math.h>
 
 #include "common.cuh"
@@ -170,6 +172,16 @@ __device__ __forceinline__ uint32_t vf_key(float x) {
 __device__ __forceinline__ float vf_unkey(uint32_t k) {
   return k == 0 ? -INFINITY : __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
+// The factor of a row's logits before the exponential: 1 / temperature, or, where the row's largest
+// logit is finite and that product is not, a power of two that brings the largest to 2^100.  Two
+// logits of such a row differ by at least 2^-24 of the largest's magnitude, far more than a
+// weight can span under either factor: equal ones weigh 1, the others 0.  (1 / temperature is
+// below 2^128, so the largest's magnitude is at least 1/2 there and the exponent in range.)
+__device__ __forceinline__ float vf_inv(float top, float inv_temp) {
+  if (fabsf(__fmul_rn(top, inv_temp)) < INFINITY || !(fabsf(top) < INFINITY)) return inv_temp;
+  const uint32_t e = (__float_as_uint(top) >> 23) & 0xffu;
+  return __uint_as_float((354u - e) << 23);
+}
 __device__ __forceinline__ int vf_drafts(const VfArgs& a, int b) {
   return a.n_draft ? min(max(a.n_draft[b], 0), a.T) : a.T;
 }
@@ -233,7 +245,8 @@ __device__ __forceinline__ VfSeq vf_decide(const VfArgs& a, int b, float* prob) 
     } else if (r.drafted) {
       {
         VfFix f;
-        const float w = f.add(vf_exp(r.logit, a.inv_temp, __fmul_rn(vf_unkey(r.top), a.inv_temp)));
+        const float top = vf_unkey(r.top), inv = vf_inv(top, a.inv_temp);
+        const float w = f.add(vf_exp(r.logit, inv, __fmul_rn(top, inv)));
         const float p = r.sum ? __fdiv_rn(w, (float)r.sum * 0x1p-40f) : 0.f;
         ok = __fmul_rn(a.u[(int64_t)b * (a.T + 1) + lane], r.q) < p;
         *prob = r.q > 0.f ? fminf(__fdiv_rn(p, r.q), 1.f) : p > 0.f ? 1.f : 0.f;
@@ -263,8 +276,9 @@ struct VfDraw {
     q = s.refused && a.probs ? a.probs + ((int64_t)b * a.T + s.accepted) * a.V : nullptr;
     q_vec = ((reinterpret_cast<uintptr_t>(q) - vec.skew * 4) & 15u) == 0;
     z = (float)s.row.sum * 0x1p-40f;
-    inv_temp = a.inv_temp;
-    mx = __fmul_rn(vf_unkey(s.row.top), a.inv_temp);
+    const float top = vf_unkey(s.row.top);
+    inv_temp = vf_inv(top, a.inv_temp);
+    mx = __fmul_rn(top, inv_temp);
   }
   // adds the weights of vector j to f; `each`: the running sums after every element
   __device__ __forceinline__ void weigh(int j, VfFix& f, unsigned long long* each) const {
@@ -341,7 +355,7 @@ __device__ __forceinline__ void vf_pick(const VfArgs& a, int b, const VfSeq& s, 
     if (!a.probs && s.refused && s.row.drafted) {  // without the refused token
       if (tid == 0) {
         VfFix f;
-        f.add(vf_exp(s.row.logit, a.inv_temp, draw.mx));
+        f.add(vf_exp(s.row.logit, draw.inv_temp, draw.mx));
         steps[(draw.id + draw.vec.skew) / N / 32] -= f.sum();
       }
       __syncthreads();
@@ -425,7 +439,7 @@ __global__ void __launch_bounds__(kVfThreads) k_verify_sum(VfArgs a) {
   VfRow* row = a.rows + blockIdx.y;
   const VfVec<E> vec((const E*)a.logits + (int64_t)blockIdx.y * a.row_stride, a.V);
   // rounding is monotonic: the largest product is the largest logit's
-  const float mx = __fmul_rn(vf_unkey(row->top), a.inv_temp);
+  const float top = vf_unkey(row->top), inv_temp = vf_inv(top, a.inv_temp), mx = __fmul_rn(top, inv_temp);
   const int lane = threadIdx.x & 31, first = blockIdx.x * kVfThreads * a.per;
   if (fabsf(mx) < INFINITY) {
     VfFix f;
@@ -437,7 +451,7 @@ __global__ void __launch_bounds__(kVfThreads) k_verify_sum(VfArgs a) {
         float x[N];
         vec.unpack(vec.load(j), x);
 #pragma unroll
-        for (int e = 0; e < N; ++e) f.add(vf_exp(x[e], a.inv_temp, mx));
+        for (int e = 0; e < N; ++e) f.add(vf_exp(x[e], inv_temp, mx));
       }
       if (kDraw) {
         const unsigned long long y = f.warp_sum();

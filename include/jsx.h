@@ -503,7 +503,8 @@ int jsx_pages_compact(const int32_t* table, const int32_t* held, const int32_t* 
  * ids outside [0, V).  temperature 0: greedy (p = 1 at the first maximum; uniforms
  * may be NULL).  Sums are over integers (weights of 2^-40), so the tokens do not
  * depend on the order of execution.  NaN logits have no mass; a row without a
- * finite maximum accepts nothing and draws -1.  0 <= T <= 31, V <= 2^20,
+ * finite maximum accepts nothing and draws -1 (a finite one counts also where its
+ * quotient by the temperature overflows: the mass is then with its equals).  0 <= T <= 31, V <= 2^20,
  * B (T + 1) <= 65535.  workspace: jsx_verify_workspace_size bytes, 16-byte aligned,
  * zero-filled once and zero again after every call: calls of other shapes that follow
  * one another may share the largest one's, calls that run at the same time may not. */

@@ -174,13 +174,16 @@ def pages_compact(table, held, refs):
 
 # ---- drafted tokens ----
 def _weights(row, inv_temp):
-    """Integer weights of one row of logits (float32 products, 64-bit exponentials)."""
+    """Integer weights of one row of logits (float32 products, 64-bit exponentials; products in
+    64 bits where the largest logit's is finite only there)."""
     with np.errstate(invalid="ignore", over="ignore"):
-        x = (row.astype(np.float32) * np.float32(inv_temp)).astype(np.float64)
-        x = np.where(np.isnan(x), -np.inf, x)
-        m = x.max()
-        if not np.isfinite(m):
+        row = np.where(np.isnan(row), -np.inf, row).astype(np.float32)
+        if not np.isfinite(row.max()):
             return None
+        x = (row * np.float32(inv_temp)).astype(np.float64)
+        if not np.isfinite(x.max()):
+            x = row.astype(np.float64) * np.float64(inv_temp)
+        m = x.max()
         return np.floor(np.exp(x - m) * 2.0 ** 40).astype(np.int64)
 
 
