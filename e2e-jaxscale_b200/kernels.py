@@ -8,6 +8,7 @@ torch is the allocator and stream provider, the arithmetic is in libjsx.so.
 from __future__ import annotations
 
 import ctypes
+import weakref
 
 import torch
 
@@ -55,9 +56,19 @@ def pdl_enabled() -> bool:
 def device_error() -> int:
     """jsx_device_error: JSX_ETIMEDOUT (3) when a bounded wait of the whole-step kernel,
     the streaming GEMV, the tensor-core projections or the attention over 4-bit pages gave up
-    since the last call, else 0 (reads and clears the error words; synchronous)."""
+    since the last call, else 0 (reads and clears the error words; synchronous).  Then the
+    workspaces of kv4_attn_workspace are zero-filled again: the call that gave up may have left
+    counters of parts that were never joined, which a later call would take for its own."""
     out = ctypes.c_int(0)
     call("jsx_device_error", ctypes.byref(out))
+    if out.value:
+        stale = list(_attn_workspaces.values())
+        for dev in {ws.device for ws in stale if ws.is_cuda}:
+            torch.cuda.synchronize(dev)   # (other streams may still use theirs)
+        for ws in stale:
+            ws.zero_()
+        for dev in {ws.device for ws in stale if ws.is_cuda}:
+            torch.cuda.synchronize(dev)
     return out.value
 
 
@@ -571,10 +582,15 @@ def kv4_read(pool, table, positions, k, v, tokens_per_seq=1, n_tokens=None):
          tokens_per_seq, nkv, hd, pt, _stream())
 
 
+_attn_workspaces = weakref.WeakValueDictionary()  # those alive, for device_error
+
+
 def kv4_attn_workspace(B, T, nq, nkv, head_dim, device) -> torch.Tensor:
     n = ctypes.c_size_t(0)
     call("jsx_kv4_attn_workspace_size", B, T, nq, nkv, head_dim, ctypes.byref(n))
-    return torch.zeros(n.value, dtype=torch.uint8, device=device)
+    ws = torch.zeros(n.value, dtype=torch.uint8, device=device)
+    _attn_workspaces[id(ws)] = ws
+    return ws
 
 
 def kv4_attn(q, pool, table, positions, head_dim, workspace, scale=None, tokens_per_seq=1, n_tokens=None, window=0,

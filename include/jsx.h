@@ -56,7 +56,8 @@ int jsx_get_launch_flags(void);
 /* Reads and clears the device error words of the streaming GEMV, of the
  * whole-step kernel, of the tensor-core projections and of jsx_kv4_attn: a bounded pipeline or
  * grid-barrier wait that gave up (the kernel then finished without its
- * result) reports JSX_ETIMEDOUT.
+ * result) reports JSX_ETIMEDOUT.  A workspace that has to be zero-filled once is to be
+ * zero-filled again after that: the call that gave up may have left counters in it.
  * Synchronous (a device copy). */
 int jsx_device_error(int* status);
 
@@ -447,9 +448,9 @@ int jsx_kv4_read(const void* pool, int num_pages, const int32_t* page_table, int
  * j < sinks); out = softmax(scale q.k) v over the visible rows, 0 when there is
  * none.  q and out [B * T][nq][head_dim] bf16 with token strides q_stride and
  * out_stride (elements, multiples of 8); query head h reads kv head h / (nq / nkv).
- * workspace: jsx_kv4_attn_workspace_size bytes, 16-byte aligned, zero-filled once.
- * Calls of other shapes that follow one another may share the largest one's; calls
- * that run at the same time may not. */
+ * workspace: jsx_kv4_attn_workspace_size bytes, 16-byte aligned, zero-filled once,
+ * and again after jsx_device_error reported JSX_ETIMEDOUT.  Calls of other shapes that
+ * follow one another may share the largest one's; calls that run at the same time may not. */
 int jsx_kv4_attn_workspace_size(int B, int T, int nq, int nkv, int head_dim, size_t* bytes);
 int jsx_kv4_attn(const void* q, int64_t q_stride, const void* pool, int num_pages,
                  const int32_t* page_table, int table_slots, const int32_t* positions,
