@@ -585,10 +585,16 @@ def kv4_read(pool, table, positions, k, v, tokens_per_seq=1, n_tokens=None):
 _attn_workspaces = weakref.WeakValueDictionary()  # those alive, for device_error
 
 
-def kv4_attn_workspace(B, T, nq, nkv, head_dim, device) -> torch.Tensor:
+def kv4_attn_workspace_bytes(B, T, nq, nkv, head_dim) -> int:
     n = ctypes.c_size_t(0)
     call("jsx_kv4_attn_workspace_size", B, T, nq, nkv, head_dim, ctypes.byref(n))
-    ws = torch.zeros(n.value, dtype=torch.uint8, device=device)
+    return n.value
+
+
+def kv4_attn_workspace(B, T, nq, nkv, head_dim, device, at_least=0) -> torch.Tensor:
+    """A workspace of kv4_attn for this shape, and for every other one that needs no more bytes."""
+    size = max(kv4_attn_workspace_bytes(B, T, nq, nkv, head_dim), at_least)
+    ws = torch.zeros(size, dtype=torch.uint8, device=device)
     _attn_workspaces[id(ws)] = ws
     return ws
 
