@@ -25,11 +25,14 @@ class PagedKV4Cache:
         i32 = dict(dtype=torch.int32, device=device)
         self.pool = torch.zeros(num_layers, self.num_pages, num_kv_heads, page_bytes // num_kv_heads,
                                 dtype=torch.uint8, device=device)
-        self.table = torch.full((batch_size, self.slots), -1, **i32)
-        self.held = torch.zeros(batch_size, **i32)
+        # table and held are parts of one buffer, so that fork sets aside both in one copy
+        n = batch_size * self.slots
+        self._rows, self._old_rows = (torch.full((n + batch_size,), -1, **i32) for _ in range(2))
+        self.table, self.held, self._old_table, self._old_held = (
+            part for rows in (self._rows, self._old_rows) for part in (rows[:n].view(batch_size, self.slots), rows[n:]))
+        self.held.zero_()
         self.refs = torch.zeros(self.num_pages, **i32)
         self.missing = torch.zeros(1, **i32)
-        self._spare = torch.empty_like(self.table), torch.empty_like(self.held)
         self._remap = torch.empty_like(self.refs)
         self._ws = K.pages_workspace(batch_size, self.slots, self.num_pages, device)
         self._attn_ws = {}       # by stream: its workspace, of the largest call so far
@@ -39,18 +42,17 @@ class PagedKV4Cache:
     # ---- pages ----
     def reserve(self, keep: torch.Tensor, need: torch.Tensor) -> torch.Tensor:
         """Every sequence keeps its first keep[b] tokens (no more than its pages hold) and gets pages
-        of its own from there to token need[b] - 1; the rest goes back.  Returns `missing` (int32 [1] on the device):
-        0, or how many pages there were too few; nothing is changed then."""
+        of its own from there to token need[b] - 1; the rest goes back.  Returns `missing` (int32 [1]
+        on the device): 0, or how many pages there were too few; nothing is changed then."""
         return K.pages_resize(self.table, self.held, self.refs, keep, need, self.pool, self.page_tokens, self._ws,
                               missing=self.missing)
 
     def fork(self, parent: torch.Tensor) -> None:
         """Sequence b goes on from sequence parent[b] (-1: empty).  Pages are shared until they are
-        written; `table` and `held` are other tensors afterwards."""
-        t, h = self._spare
-        K.pages_fork(self.table, self.held, self.refs, parent, table_out=t, held_out=h, refs_out=self.refs)
-        self._spare = self.table, self.held
-        self.table, self.held = t, h
+        written.  `table`, `held` and `refs` are changed in place, for the graphs that read them."""
+        self._old_rows.copy_(self._rows)
+        K.pages_fork(self._old_table, self._old_held, self.refs, parent, table_out=self.table, held_out=self.held,
+                     refs_out=self.refs)
 
     def compact(self) -> torch.Tensor:
         """Live pages move to the lowest numbers; returns the new number of every old one (-1: free)."""
