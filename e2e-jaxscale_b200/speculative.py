@@ -190,7 +190,8 @@ def speculative_generate(model: GLM4ForCausalLM, input_ids, max_new_tokens: int 
     while not all(over(b) for b in range(B)):
         drafts = [[] if over(b) else list(draft(history[b], min(draft_tokens, max_new_tokens - len(out[b]) - 1)))
                   for b in range(B)]
-        first = torch.tensor([len(h) - 1 for h in history], dtype=torch.int32)
+        # (a sequence that is over keeps nothing: its pages are free for the others)
+        first = torch.tensor([0 if over(b) else len(history[b]) - 1 for b in range(B)], dtype=torch.int32)
         count = torch.tensor([0 if over(b) else 1 + len(drafts[b]) for b in range(B)], dtype=torch.int32)
         fed = torch.tensor([[history[b][-1]] + drafts[b] + [0] * (draft_tokens - len(drafts[b])) for b in range(B)],
                            dtype=torch.int32)
