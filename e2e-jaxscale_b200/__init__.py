@@ -13,6 +13,6 @@ from .flash import GLM4FlashForCausalLM  # noqa: F401
 from .layers.paged_cache import PagedKV4Cache  # noqa: F401
 from .mesh import Comm, Mesh, create_mesh  # noqa: F401
 from .runner import JittedModel, greedy_generate, sample_generate  # noqa: F401
-from .speculative import speculative_generate  # noqa: F401
+from .speculative import PoolExhausted, speculative_generate  # noqa: F401
 
 __version__ = "0.1.0"

@@ -145,10 +145,17 @@ def _head(model, h, ws, ids, logits) -> None:
                            ids[m], ws, logits[m])
 
 
+class PoolExhausted(RuntimeError):
+    """The page pool cannot hold the next step.  `tokens`: what speculative_generate had until then,
+    in the shape that it returns."""
+
+    tokens: torch.Tensor | None = None
+
+
 def _reserve(st: DraftedState, keep, need) -> None:
     missing = int(st.cache.reserve(keep, need))
     if missing:
-        raise RuntimeError(f"the page pool is too small: {missing} pages missing")
+        raise PoolExhausted(f"the page pool is too small: {missing} pages missing")
 
 
 def speculative_generate(model: GLM4ForCausalLM, input_ids, max_new_tokens: int = 128, draft_tokens: int = 4,
@@ -159,7 +166,8 @@ def speculative_generate(model: GLM4ForCausalLM, input_ids, max_new_tokens: int 
     draft(history, count) -> at most count token ids; temperature 0 is greedy.  Sequences go on
     until max_new_tokens or an EOS id, each at its own pace.  Returns [B, prompt + max_new_tokens]
     int32 on the host, filled up with the EOS id (or -1) after a sequence's end.  `stats`
-    receives the steps taken and the drafts proposed and accepted."""
+    receives the steps taken and the drafts proposed and accepted.  Where num_pages do not
+    suffice, PoolExhausted has the text so far."""
     ids = torch.as_tensor(input_ids, dtype=torch.int32)
     B, S = ids.shape
     T, V, dev = draft_tokens + 1, model.config.vocab_size, model.device
@@ -179,39 +187,46 @@ def speculative_generate(model: GLM4ForCausalLM, input_ids, max_new_tokens: int 
     def over(b):
         return len(out[b]) >= max_new_tokens or (len(out[b]) > 0 and out[b][-1] in eos)
 
-    # the first token: a draw without drafts
-    logits = prefill(model, st, ids.to(dev), window, sinks)
-    none = torch.zeros(B, 0, dtype=torch.int32, device=dev)
-    _, tokens, _ = K.verify_drafts(logits[:, None], none, torch.rand(B, 1, generator=gen, device=dev),
-                                   K.verify_workspace(B, 0, V, dev), temperature=temperature)
-    for b, row in enumerate(tokens.tolist()):
-        take(b, row)
+    def text():
+        fill = eos[0] if eos else -1
+        rows = [out[b] + [fill] * (max_new_tokens - len(out[b])) for b in range(B)]
+        return torch.cat([ids, torch.tensor(rows, dtype=torch.int32).reshape(B, max_new_tokens)], dim=1)
 
-    while not all(over(b) for b in range(B)):
-        drafts = [[] if over(b) else list(draft(history[b], min(draft_tokens, max_new_tokens - len(out[b]) - 1)))
-                  for b in range(B)]
-        # (a sequence that is over keeps nothing: its pages are free for the others)
-        first = torch.tensor([0 if over(b) else len(history[b]) - 1 for b in range(B)], dtype=torch.int32)
-        count = torch.tensor([0 if over(b) else 1 + len(drafts[b]) for b in range(B)], dtype=torch.int32)
-        fed = torch.tensor([[history[b][-1]] + drafts[b] + [0] * (draft_tokens - len(drafts[b])) for b in range(B)],
-                           dtype=torch.int32)
-        st.first.copy_(first)
-        st.count.copy_(count)
-        st.ids.copy_(fed.reshape(-1))
-        _reserve(st, st.first, st.first + st.count)
-        logits = step(model, st, window, sinks)
-        accepted, tokens, _ = K.verify_drafts(
-            logits, st.ids.view(B, T)[:, 1:].contiguous(), torch.rand(B, T, generator=gen, device=dev), st.verify_ws,
-            n_draft=(st.count - 1).clamp_(min=0), temperature=temperature)
-        accepted, tokens = accepted.tolist(), tokens.tolist()
-        tally["steps"] += 1
-        for b in range(B):
-            if not over(b):
-                tally["drafted"] += len(drafts[b])
-                tally["accepted"] += accepted[b]
-                take(b, tokens[b][:accepted[b] + 1])
+    try:
+        # the first token: a draw without drafts
+        logits = prefill(model, st, ids.to(dev), window, sinks)
+        none = torch.zeros(B, 0, dtype=torch.int32, device=dev)
+        _, tokens, _ = K.verify_drafts(logits[:, None], none, torch.rand(B, 1, generator=gen, device=dev),
+                                       K.verify_workspace(B, 0, V, dev), temperature=temperature)
+        for b, row in enumerate(tokens.tolist()):
+            take(b, row)
+
+        while not all(over(b) for b in range(B)):
+            drafts = [[] if over(b) else list(draft(history[b], min(draft_tokens, max_new_tokens - len(out[b]) - 1)))
+                      for b in range(B)]
+            # (a sequence that is over keeps nothing: its pages are free for the others)
+            first = torch.tensor([0 if over(b) else len(history[b]) - 1 for b in range(B)], dtype=torch.int32)
+            count = torch.tensor([0 if over(b) else 1 + len(drafts[b]) for b in range(B)], dtype=torch.int32)
+            fed = torch.tensor([[history[b][-1]] + drafts[b] + [0] * (draft_tokens - len(drafts[b])) for b in range(B)],
+                               dtype=torch.int32)
+            st.first.copy_(first)
+            st.count.copy_(count)
+            st.ids.copy_(fed.reshape(-1))
+            _reserve(st, st.first, st.first + st.count)
+            logits = step(model, st, window, sinks)
+            accepted, tokens, _ = K.verify_drafts(
+                logits, st.ids.view(B, T)[:, 1:].contiguous(), torch.rand(B, T, generator=gen, device=dev),
+                st.verify_ws, n_draft=(st.count - 1).clamp_(min=0), temperature=temperature)
+            accepted, tokens = accepted.tolist(), tokens.tolist()
+            tally["steps"] += 1
+            for b in range(B):
+                if not over(b):
+                    tally["drafted"] += len(drafts[b])
+                    tally["accepted"] += accepted[b]
+                    take(b, tokens[b][:accepted[b] + 1])
+    except PoolExhausted as e:
+        e.tokens = text()
+        raise
     if stats is not None:
         stats.update(tally)
-    fill = eos[0] if eos else -1
-    rows = [out[b] + [fill] * (max_new_tokens - len(out[b])) for b in range(B)]
-    return torch.cat([ids, torch.tensor(rows, dtype=torch.int32).reshape(B, max_new_tokens)], dim=1)
+    return text()

@@ -57,3 +57,16 @@ def test_cache_of_finished_sequences_is_empty(jsx, model, monkeypatch):
     jsx.speculative_generate(model, p, seed=seed, eos_token_id=eos, **KW)
     assert any(count[0] == 0 for count, _ in seen)
     assert all(held[0] == 0 for count, held in seen if count[0] == 0)
+
+
+def test_the_text_survives_a_pool_that_runs_out(jsx, model):
+    p = prompts(2, 16)
+    whole = jsx.speculative_generate(model, p, seed=3, **KW)
+    with pytest.raises(RuntimeError, match="pages missing") as e:
+        jsx.speculative_generate(model, p, seed=3, num_pages=5, **KW)
+    text = e.value.tokens                          # 5 pages: 32 tokens of both are stored
+    assert text.shape == whole.shape and text.dtype == torch.int32
+    assert torch.equal(text[:, :33], whole[:, :33]) and (text[:, 33:] == -1).all()
+    with pytest.raises(RuntimeError) as e:         # not even the prompt fits
+        jsx.speculative_generate(model, p, num_pages=1, **KW)
+    assert torch.equal(e.value.tokens[:, :16], torch.as_tensor(p, dtype=torch.int32)) and (e.value.tokens[:, 16:] == -1).all()
