@@ -168,7 +168,7 @@ def speculative_generate(model: GLM4ForCausalLM, input_ids, max_new_tokens: int 
     int32 on the host, filled up with the EOS id (or -1) after a sequence's end.  `stats`
     receives the steps taken and the drafts proposed and accepted.  Where num_pages do not
     suffice, PoolExhausted has the text so far."""
-    ids = torch.as_tensor(input_ids, dtype=torch.int32)
+    ids = torch.as_tensor(input_ids, dtype=torch.int32).cpu()
     B, S = ids.shape
     T, V, dev = draft_tokens + 1, model.config.vocab_size, model.device
     eos = [] if eos_token_id is None else [eos_token_id] if isinstance(eos_token_id, int) else list(eos_token_id)

@@ -1,4 +1,4 @@
-"""speculative_generate when pages are scarce."""
+"""speculative_generate when pages are scarce, and with prompts on the GPU."""
 
 import importlib
 
@@ -70,3 +70,10 @@ def test_the_text_survives_a_pool_that_runs_out(jsx, model):
     with pytest.raises(RuntimeError) as e:         # not even the prompt fits
         jsx.speculative_generate(model, p, num_pages=1, **KW)
     assert torch.equal(e.value.tokens[:, :16], torch.as_tensor(p, dtype=torch.int32)) and (e.value.tokens[:, 16:] == -1).all()
+
+
+def test_prompts_on_the_gpu(jsx, model):
+    p = torch.from_numpy(prompts(2, 9)).int()
+    a = jsx.speculative_generate(model, p, max_new_tokens=6)
+    b = jsx.speculative_generate(model, p.cuda(), max_new_tokens=6)
+    assert not b.is_cuda and torch.equal(a, b)
