@@ -45,6 +45,19 @@ def _opt(t, name, dtype=BF16):
     return None if t is None else _need(t, name, dtype)
 
 
+def _strides(t):
+    """Strides in elements.  A dimension of length one has none of its own (torch leaves any number
+    there): it gets the one that a dense tensor of the inner dimensions has."""
+    st = t.stride()
+    if 1 in t.shape:
+        st = list(st)
+        for d in range(len(st) - 1, -1, -1):
+            if t.shape[d] == 1:
+                st[d] = st[d + 1] * t.shape[d + 1] if d + 1 < len(st) else 1
+        st = tuple(st)
+    return st
+
+
 def set_pdl(enabled: bool) -> None:
     call("jsx_set_launch_flags", JSX_LAUNCH_PDL if enabled else 0)
 
@@ -545,11 +558,11 @@ def kv4_page_bytes(nkv, head_dim, page_tokens) -> int:
 def _kv4_rows(k, v, B, T, nkv):
     """Strides and cache rows of k and v: [B, L, nkv, hd] (a static cache, rows by position) or
     [B * T, nkv, hd] (one row per token; the tokens may be strided, as slices of a fused q/k/v are)."""
-    if k.shape != v.shape or k.stride() != v.stride() or k.dtype != BF16 or v.dtype != BF16:
+    st = _strides(k)
+    if k.shape != v.shape or st != _strides(v) or k.dtype != BF16 or v.dtype != BF16:
         raise ValueError("k and v must be bf16 of one shape and layout")
     if not (k.is_cuda and v.is_cuda):
         raise ValueError("k and v must be CUDA tensors")
-    st = k.stride()
     if st[-1] != 1 or k.shape[-2] != nkv:
         raise ValueError(f"rows must be [{nkv} kv heads, head_dim] with unit stride")
     if k.dim() == 4:
@@ -615,8 +628,8 @@ def kv4_attn(q, pool, table, positions, head_dim, workspace, scale=None, tokens_
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != BF16 or out.stride(1) != 1 or not out.is_cuda:
         raise ValueError("out must be a bf16 CUDA tensor of q's shape")
-    call("jsx_kv4_attn", q.data_ptr(), q.stride(0), pool.data_ptr(), P_, table.data_ptr(), slots, positions.data_ptr(),
-         None if n_tokens is None else n_tokens.data_ptr(), out.data_ptr(), out.stride(0), B, T,
+    call("jsx_kv4_attn", q.data_ptr(), _strides(q)[0], pool.data_ptr(), P_, table.data_ptr(), slots, positions.data_ptr(),
+         None if n_tokens is None else n_tokens.data_ptr(), out.data_ptr(), _strides(out)[0], B, T,
          q.shape[1] // head_dim, nkv, head_dim, pt, window, sinks, head_dim ** -0.5 if scale is None else scale,
          workspace.data_ptr(), workspace.numel(), _stream())
     return out
@@ -713,7 +726,9 @@ def verify_drafts(logits, draft_ids, uniforms, workspace, draft_probs=None, n_dr
     if logits.dim() != 3 or not logits.is_cuda or logits.dtype not in (BF16, torch.float32):
         raise ValueError("logits must be a [B, T + 1, V] bf16 or f32 CUDA tensor")
     B, T, V = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
-    sb, sr, sv = logits.stride()
+    sb, sr, sv = _strides(logits)
+    if T == 0:
+        sr = sb  # one row per sequence: sequences are what is spaced
     if sv != 1 or (B > 1 and sb != sr * (T + 1)):
         raise ValueError("logits rows must be evenly spaced, with unit stride in a row")
     _need(draft_ids, "draft_ids", I32)
