@@ -45,19 +45,6 @@ def _opt(t, name, dtype=BF16):
     return None if t is None else _need(t, name, dtype)
 
 
-def _strides(t):
-    """Strides in elements.  A dimension of length one has none of its own (torch leaves any number
-    there): it gets the one that a dense tensor of the inner dimensions has."""
-    st = t.stride()
-    if 1 in t.shape:
-        st = list(st)
-        for d in range(len(st) - 1, -1, -1):
-            if t.shape[d] == 1:
-                st[d] = st[d + 1] * t.shape[d + 1] if d + 1 < len(st) else 1
-        st = tuple(st)
-    return st
-
-
 def set_pdl(enabled: bool) -> None:
     call("jsx_set_launch_flags", JSX_LAUNCH_PDL if enabled else 0)
 
@@ -555,11 +542,23 @@ def kv4_page_bytes(nkv, head_dim, page_tokens) -> int:
     return n.value
 
 
+def _dense_ones(shape, st):
+    """Strides with those of dimensions of length one (where torch leaves any number) as a dense tensor
+    has them."""
+    st = list(st)
+    for d in range(len(st) - 1, -1, -1):
+        if shape[d] == 1:
+            st[d] = st[d + 1] * shape[d + 1] if d + 1 < len(st) else 1
+    return tuple(st)
+
+
 def _kv4_rows(k, v, B, T, nkv):
     """Strides and cache rows of k and v: [B, L, nkv, hd] (a static cache, rows by position) or
     [B * T, nkv, hd] (one row per token; the tokens may be strided, as slices of a fused q/k/v are)."""
-    st = _strides(k)
-    if k.shape != v.shape or st != _strides(v) or k.dtype != BF16 or v.dtype != BF16:
+    shape, st, sv = k.shape, k.stride(), v.stride()
+    if 1 in shape and shape == v.shape and (st != sv or any(x % 8 for x in st[:-1])):
+        st, sv = _dense_ones(shape, st), _dense_ones(shape, sv)
+    if shape != v.shape or st != sv or k.dtype != BF16 or v.dtype != BF16:
         raise ValueError("k and v must be bf16 of one shape and layout")
     if not (k.is_cuda and v.is_cuda):
         raise ValueError("k and v must be CUDA tensors")
@@ -628,10 +627,11 @@ def kv4_attn(q, pool, table, positions, head_dim, workspace, scale=None, tokens_
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != BF16 or out.stride(1) != 1 or not out.is_cuda:
         raise ValueError("out must be a bf16 CUDA tensor of q's shape")
-    call("jsx_kv4_attn", q.data_ptr(), _strides(q)[0], pool.data_ptr(), P_, table.data_ptr(), slots, positions.data_ptr(),
-         None if n_tokens is None else n_tokens.data_ptr(), out.data_ptr(), _strides(out)[0], B, T,
-         q.shape[1] // head_dim, nkv, head_dim, pt, window, sinks, head_dim ** -0.5 if scale is None else scale,
-         workspace.data_ptr(), workspace.numel(), _stream())
+    width = q.shape[1]
+    call("jsx_kv4_attn", q.data_ptr(), q.stride(0) if B * T > 1 else width, pool.data_ptr(), P_, table.data_ptr(),
+         slots, positions.data_ptr(), None if n_tokens is None else n_tokens.data_ptr(), out.data_ptr(),
+         out.stride(0) if B * T > 1 else width, B, T, width // head_dim, nkv, head_dim, pt, window, sinks,
+         head_dim ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel(), _stream())
     return out
 
 
@@ -677,8 +677,8 @@ def pages_fork(table, held, refs, parent, table_out=None, held_out=None, refs_ou
 
 def pages_resize(table, held, refs, keep, need, pool, page_tokens, workspace, missing=None):
     """In place: row b keeps its first keep[b] tokens (no more than its pages hold) and has pages
-    of its own from there up to need[b] (include/jsx.h jsx_pages_resize).  Returns missing, int32 [1] on the device: 0, or how many
-    pages there were too few (nothing is changed then)."""
+    of its own from there up to need[b] (include/jsx.h jsx_pages_resize).  Returns missing, int32 [1] on
+    the device: 0, or how many pages there were too few (nothing is changed then)."""
     S, slots, P_ = _pages(table, held, refs)
     _need(keep, "keep", I32)
     _need(need, "need", I32)
@@ -726,10 +726,10 @@ def verify_drafts(logits, draft_ids, uniforms, workspace, draft_probs=None, n_dr
     if logits.dim() != 3 or not logits.is_cuda or logits.dtype not in (BF16, torch.float32):
         raise ValueError("logits must be a [B, T + 1, V] bf16 or f32 CUDA tensor")
     B, T, V = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
-    sb, sr, sv = _strides(logits)
-    if T == 0:
-        sr = sb  # one row per sequence: sequences are what is spaced
-    if sv != 1 or (B > 1 and sb != sr * (T + 1)):
+    sb, sr, sv = logits.stride()
+    if T == 0:  # one row per sequence: the sequences' spacing is the rows'
+        sr = sb if B > 1 else V
+    if (sv != 1 and V > 1) or (B > 1 and sb != sr * (T + 1)):
         raise ValueError("logits rows must be evenly spaced, with unit stride in a row")
     _need(draft_ids, "draft_ids", I32)
     _opt(uniforms, "uniforms", torch.float32)
