@@ -610,7 +610,10 @@ static int64_t ka_chunks(int64_t table_rows, int T, int window, int sinks) {
 //     8: 70 / 45, 16: 130 / 64, 64: 490 / 198;  5 with counts of 0 to 5: 36 / 42
 //   8 heads on 1, 64 sequences of up to 4000 rows: T 5: 36 / 39, 9: 51 / 42, 16: 76 / 47
 //   32 heads on 2, one sequence of 4000 rows: T 8: 17 / 23, 33: 29 / 34, 64: 44 / 34
-// Up to 48 query rows per kv head it never does.
+// Up to 48 query rows per kv head it never does.  The lengths are on the device, so the chunks are
+// those of the table's capacity (or the window): short sequences in a long table may get the
+// 128-row kernel and its 20 us.  head_dim 64 has the 16-row kernel alone (64 tokens of 16 sequences
+// of up to 8191 rows: 328 us; a prompt of 8192 tokens with a window of 4096: 1576 us).
 static bool ka_wide_ever(int T, int nq, int nkv, int head_dim) { return head_dim == 128 && (int64_t)(nq / nkv) * T > 3 * kKaRows; }
 static bool ka_wide(int B, int T, int nq, int nkv, int head_dim, bool counts, int64_t chunks) {
   if (!ka_wide_ever(T, nq, nkv, head_dim)) return false;

@@ -24,11 +24,12 @@
 // A stored value is exact in f16, q is scaled by a power of two per row, P has 11 bits: the
 // same roundings as the 16-row kernel's.
 //
-// Bound: the softmax warps, two per scheduler, which are busy all the time: 64 exponentials,
-// their conversions and sums take 1300 cycles of a step's 2700 and share the issue slots (55%
-// taken) with the conversions; an item's first rows and its end cost about 6 us a CTA, the
+// Bound: the two groups of softmax warps, two warps per scheduler, not the products.  A group's
+// step takes 2700 cycles, 1300 of them for 64 exponentials, their conversions and sums, and shares
+// the issue slots (55% taken) with the conversions of codes; an item's first rows and its end cost about 6 us a CTA, the
 // joining launch 7.  32 heads on 2, 16 sequences of up to 8191 rows: 41 us for 5 tokens, 64 for
-// 16, 198 for 64 (the 16-row kernel: 48, 130, 490), which is 0.45 PFLOP/s at 64.
+// 16, 198 for 64 (the 16-row kernel: 48, 130, 490), which is 0.45 PFLOP/s at 64; a prompt of
+// 8192 tokens with a window of 4096: 980 us, 0.42 PFLOP/s.
 //
 // NaN: a row's NaN scale enters V as 0 (it would reach every query row through weights of
 // 0) and is noted; the query rows that see it get their NaN when they are written.

@@ -24,9 +24,10 @@
 // crossing and weighs it again.  Slices meet in integer atomics (maximum, sum), so they need no
 // order and no wait; the second pass over the logits comes from L2 (at most 126 MB of it).
 // Bound: from some 20 rows on the exponentials' instructions (18 per logit with the exact
-// sum, 75% of the issue slots) rather than the bytes; launches below.  32 x 5 rows of 151552
-// with draft distributions: 44 us, 12 of them the maxima (4.0 TB/s) and 21 the sums; 1 x 5
-// without: 13.0 us; 16 x 8 rows of 32003, greedy: 5.8 us (7.9 in three launches, which also
+// sum, 75% of the issue slots) rather than the bytes; launches below.  32 sequences of up
+// to 5 rows of 151552 (129 with their counts) with draft distributions: 44 us, 12 of them the
+// maxima (39.1 MB, 3.2 TB/s) and 21 the sums (19.6 million exponentials); 1 x 5
+// without: 13.0 us; 16 x up to 8 rows (81) of 32003, greedy: 5.8 us (7.9 in three launches, which also
 // cost the host 5 us more).  One cluster per row with distributed shared memory instead of
 // atomics: 79 us; one cooperative launch in which the slices wait for one another: 17.7 against
 // 13.5 us at 1 x 5.

@@ -2,10 +2,15 @@
 
 Where the reference decodes one token per step over a static bf16 cache (runner.py:240-308,
 :366-460), a step here takes every sequence's last token and up to `draft_tokens` proposed
-ones through the model at once: the weights are read once for all of them, and the rows go
-through the tensor-core projections (jsx_tc_*, 32 tokens per call).  The target's logits then
-accept or replace the proposals (jsx_verify_drafts), so the output is distributed as without
-drafts; at temperature 0 it is the greedy continuation.
+ones through the model at once, on the tensor-core projections (jsx_tc_*, 32 tokens per call).
+Up to 32 tokens of all sequences together share one pass over the weights; more go in spans of
+whole sequences, a pass each, so drafting pays for small batches (9B shape, 40 layers, context
+1024, in a graph: 1 x 5 tokens 5.1 ms, 6 x 5 5.7 ms, 16 x 5 14.2 ms, 32 x 5 26.8 ms; one token of
+32 sequences in the plain decode step: 5.4 ms, of one: 3.6 ms).  The target's logits then accept
+or replace the proposals (jsx_verify_drafts), so at a temperature (without top-k, top-p or
+penalties) the output is distributed as without drafts.  At temperature 0 it is the greedy
+continuation; different numbers of tokens per step round differently, so two near-equal logits
+may change places between a run with drafts and one without.
 
 Per layer: q/k/v + bias + RoPE into a one-layer bf16 staging cache, its new rows into the
 4-bit pages (jsx_kv4_append), attention over the pages (jsx_kv4_attn, with an optional window
