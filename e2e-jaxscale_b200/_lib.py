@@ -39,6 +39,7 @@ I64 = ctypes.c_int64
 SIGNATURES = {
     "jsx_abi_version": [],
     "jsx_device_sm_count": [P],
+    "jsx_stream_capture_id": [P, P],
     "jsx_set_launch_flags": [I],
     "jsx_get_launch_flags": [],
     "jsx_device_error": [P],

@@ -60,6 +60,15 @@ extern "C" int jsx_device_sm_count(int* out) {
   return JSX_OK;
 }
 
+extern "C" int jsx_stream_capture_id(void* stream, uint64_t* id) {
+  JSX_REQUIRE(id != nullptr, "null id");
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long capture = 0;
+  JSX_CUDA(cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &capture));
+  *id = status == cudaStreamCaptureStatusActive ? capture : 0;
+  return JSX_OK;
+}
+
 extern "C" int jsx_set_launch_flags(int flags) {
   JSX_REQUIRE((flags & ~JSX_LAUNCH_PDL) == 0, "unknown launch flags 0x%x", flags);
   g_launch_flags = flags;

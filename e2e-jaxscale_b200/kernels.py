@@ -29,6 +29,15 @@ def _stream():
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def capture_id() -> int:
+    """The id of the graph capture that torch's current stream takes part in, 0 when it is in none."""
+    if not torch._C._cuda_isCurrentStreamCapturing():
+        return 0
+    out = ctypes.c_uint64(0)
+    call("jsx_stream_capture_id", _stream(), ctypes.byref(out))
+    return out.value
+
+
 def _need(t, name, dtype=BF16):
     if t is None:
         raise ValueError(f"{name} is required")

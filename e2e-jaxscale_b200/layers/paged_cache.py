@@ -37,7 +37,8 @@ class PagedKV4Cache:
         self._ws = K.pages_workspace(batch_size, self.slots, self.num_pages, device)
         self._attn_ws = {}       # by stream: its workspace, of the largest call so far
         self._attn_bytes = {}    # by shape
-        self._captured = {}      # workspaces that graphs write to
+        self._captured = {}      # those that graphs write to
+        self._capture_ws = {}    # by capture and stream: made in the present capture
 
     # ---- pages ----
     def reserve(self, keep: torch.Tensor, need: torch.Tensor) -> torch.Tensor:
@@ -74,24 +75,36 @@ class PagedKV4Cache:
     def attend(self, layer: int, q, positions, scale: float, tokens_per_seq: int = 1, n_tokens=None, window: int = 0,
                sinks: int = 0, out=None):
         """q [B * T, heads * head_dim] -> out, over the sequences' pages (kernels.kv4_attn).  Calls on
-        different streams have different workspaces; a captured call has the one of the stream that
-        it was captured on, so graphs captured on one stream may not be replayed at the same time."""
+        different streams have different workspaces.  A captured call has the one of the stream that
+        it was captured on, if an earlier call made it large enough, else one of its graph's own:
+        graphs of the first kind may not be replayed at the same time."""
         ws = self._workspace(positions.numel(), tokens_per_seq, q.shape[1] // self.head_dim, q.device)
         return K.kv4_attn(q, self.pool[layer], self.table, positions, self.head_dim, ws, scale=scale,
                           tokens_per_seq=tokens_per_seq, n_tokens=n_tokens, window=window, sinks=sinks, out=out)
 
     def _workspace(self, B: int, T: int, nq: int, device) -> torch.Tensor:
         """The current stream's workspace, large enough for this call: calls on one stream follow one
-        another and may share it.  One that a graph was captured with outlives its replacement."""
-        shape = (B, T, nq, self.num_kv_heads, self.head_dim)
+        another and may share it."""
+        shape = (B, T, nq)
         need = self._attn_bytes.get(shape)
         if need is None:
-            need = self._attn_bytes[shape] = K.kv4_attn_workspace_bytes(*shape)
-        stream = K._stream()
+            need = self._attn_bytes[shape] = K.kv4_attn_workspace_bytes(*shape, self.num_kv_heads, self.head_dim)
+        stream, capture = K._stream(), K.capture_id()
         ws = self._attn_ws.get(stream)
-        if ws is None or ws.numel() < need:
-            # (whole megabytes: lengths near one another need a few bytes more or less)
-            ws = self._attn_ws[stream] = K.kv4_attn_workspace(*shape, device, at_least=(need + 0xfffff) >> 20 << 20)
-        if torch.cuda.is_current_stream_capturing():
-            self._captured[ws.data_ptr()] = ws
+        if ws is not None and ws.numel() >= need:
+            if capture:
+                self._captured[ws.data_ptr()] = ws   # (it outlives its replacement)
+            return ws
+        kept, key = self._attn_ws, stream
+        if capture:
+            # its zero-fill is a node of this graph, so nothing outside of the graph may rely on it
+            kept, key = self._capture_ws, (capture, stream)
+            ws = kept.get(key)
+            if ws is not None and ws.numel() >= need:
+                return ws
+            for old in [k for k in kept if k[0] != capture]:
+                del kept[old]
+        # (whole megabytes: lengths near one another need a few bytes more or less)
+        ws = kept[key] = K.kv4_attn_workspace(*shape, self.num_kv_heads, self.head_dim, device,
+                                              at_least=(need + 0xfffff) >> 20 << 20)
         return ws

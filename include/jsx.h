@@ -45,6 +45,9 @@ int jsx_abi_version(void);
 const char* jsx_last_error(void);
 /* Number of SMs of the current device (grid sizing and tests). */
 int jsx_device_sm_count(int* out);
+/* The id of the graph capture that the stream takes part in, 0 when it is in none: what a call
+ * enqueues during one (a workspace's zero-fill) happens in that graph's replays alone. */
+int jsx_stream_capture_id(void* stream, uint64_t* id);
 /* Launch flags for every later launch of this process.  JSX_LAUNCH_PDL (1):
  * programmatic dependent launch — each kernel streams its first weight tiles
  * while the previous kernel in the stream drains (default on; the JSX_PDL

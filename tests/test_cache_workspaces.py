@@ -80,3 +80,47 @@ def test_a_captured_call_outlives_growth(jsx, cuda):
         g.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want) and bool((other == 0xff).all())
+
+
+def test_a_workspace_made_in_a_capture_is_that_graphs_own(jsx, cuda, monkeypatch):
+    """Its zero-fill is a node of the graph: a second graph that is replayed first cannot rely on it."""
+    cache = filled(jsx)
+    pos = torch.full((B,), 500, dtype=torch.int32, device="cuda")
+    q = queries(1)
+    want = cache.attend(0, q, pos, HD ** -0.5)
+    used, real = [], jsx.kernels.kv4_attn
+    monkeypatch.setattr(jsx.kernels, "kv4_attn", lambda q, pool, table, pos, hd, ws, **kw: used.append(ws) or real(q, pool, table, pos, hd, ws, **kw))
+    s = torch.cuda.Stream()
+    graphs, outs = [], []
+    for _ in range(2):
+        g, o = torch.cuda.CUDAGraph(), [torch.zeros_like(want) for _ in range(3)]
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(g, stream=s):
+            for y in o:                            # several calls of a graph share one
+                cache.attend(0, q, pos, HD ** -0.5, out=y)
+        graphs.append(g)
+        outs.append(o)
+    assert len({w.data_ptr() for w in used[:3]}) == 1 and len({w.data_ptr() for w in used[3:]}) == 1
+    used[0].fill_(1)                               # as memory that nobody filled
+    torch.cuda.synchronize()
+    for g, o in zip(reversed(graphs), reversed(outs)):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want) for y in o)
+    with torch.cuda.stream(s):                     # and neither can a call outside of graphs
+        got = cache.attend(0, q, pos, HD ** -0.5)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and not used[-1][:4096].any()   # (counters)
+
+
+def test_capture_id(jsx, cuda):
+    K = jsx.kernels
+    assert K.capture_id() == 0
+    x, seen = torch.zeros(4, device="cuda"), []
+    for _ in range(2):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            seen += [K.capture_id(), K.capture_id()]
+            x.add_(1)
+    assert K.capture_id() == 0 and seen[0] == seen[1] != 0 and seen[2] == seen[3] not in (0, seen[0])
+    with pytest.raises(jsx._lib.JsxError):
+        jsx._lib.call("jsx_stream_capture_id", None, None)
